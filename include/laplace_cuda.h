@@ -47,6 +47,8 @@ extern "C" {
 #define LAPLACE_TYPE_Q8_0 8u
 #define LAPLACE_TYPE_Q4_K 12u
 #define LAPLACE_TYPE_Q6_K 14u
+/* not in Laplace's table: microscaled 4-bit floating point, see laplace_cuda_mxfp4_* */
+#define LAPLACE_TYPE_MXFP4 39u
 
 enum {
     LAPLACE_OK            = 0,
@@ -248,6 +250,40 @@ int laplace_cuda_embed_rows_dev(const uint8_t* w, uint32_t type, const int* toke
                                 float* dst, void* stream);
 int laplace_cuda_lm_head_dev(const float* x, const uint8_t* w, uint32_t type, float* y, int M, int K, int N, float softcap,
                              void* stream);
+
+/* ---- MXFP4 weights ------------------------------------------------------------------------
+ * Microscaled 4-bit floating point (ggml type 39, the reference has no such type): 32 values of a row share a power of two,
+ * a value is e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives). A GGUF block is 17 bytes: the exponent + 127 (255: the
+ * block is NaN), then 16 bytes whose low halves are values 0..15 and whose high halves values 16..31.
+ * laplace_cuda_dequantize_dev, laplace_cuda_embed_rows_dev and the GGUF loader take type 39 as they take the other types. The
+ * products run on the tensor cores' block-scaled instructions and read weights from a layout of their own, which
+ * laplace_cuda_mxfp4_pack_dev makes once, at load; laplace_cuda_gemm_dev and its kin return LAPLACE_UNSUPPORTED for type 39.
+ *
+ * laplace_cuda_mxfp4_quantize_dev: n values (a multiple of 32; x_type 0 F32, 1 F16, 30 BF16; x 16-byte aligned) -> n / 32
+ *   blocks at w (any alignment). Exponent floor(log2(largest magnitude)) - 2, values to nearest, ties to even, magnitudes
+ *   over 6 held as 6; a block with an infinity or a NaN gets exponent byte 255.
+ * laplace_cuda_mxfp4_packed_size / _pack_dev: n_experts matrices of N rows of K values (one after the other; w at any
+ *   alignment; one matrix: n_experts = 1) -> the packed layout, 128-byte aligned, 0.53 bytes per value and row tiles of 128.
+ * laplace_cuda_mxfp4_gemm_dev: y[m][j] = sum_k xq[m][k] * w[j][k], where xq holds x as MXFP8: e4m3 values and, per 32 of them,
+ *   the smallest power of two that keeps the largest magnitude within 448 times it, rounded to nearest even. Sums in fp32. A
+ *   block of x with an infinity or a NaN makes its row of y NaN, as a NaN block of the weights makes its column. M = 0 is a call without effect.
+ * laplace_cuda_mxfp4_moe_grouped_dev: the same for (token, expert) pairs, as laplace_cuda_moe_grouped_dev:
+ *   y[p][j] = sum_k xq[pair_row[p]][k] * w[pair_expert[p]][j][k]; pair_row = NULL: pair p reads row p. Pairs in any order. A
+ *   negative expert leaves its row of y untouched; an expert >= n_experts_total or a row outside [0, x_rows) does too and
+ *   makes the next laplace_cuda_sync() return LAPLACE_ERR_ARG. At most 4000 experts. n_pairs = 0 is a call without effect.
+ * K is a multiple of 32, x 16-byte aligned. Workspace: the caller's, laplace_cuda_mxfp4_workspace_size(M or n_pairs, 0 or
+ *   n_experts_total, K, N) bytes, 256-byte aligned, its contents of no consequence before or after. Calls with workspaces of
+ *   their own may overlap, in streams as in captured graphs. Results do not depend on timing: the same call gives the same bits.
+ * All pointers are device memory. */
+int    laplace_cuda_mxfp4_quantize_dev(const void* x, uint32_t x_type, uint8_t* w, long long n, void* stream);
+size_t laplace_cuda_mxfp4_packed_size(int n_experts, int N, int K);
+int    laplace_cuda_mxfp4_pack_dev(const uint8_t* w, uint8_t* packed, int n_experts, int N, int K, void* stream);
+size_t laplace_cuda_mxfp4_workspace_size(int rows, int n_experts, int K, int N);
+int    laplace_cuda_mxfp4_gemm_dev(const float* x, const uint8_t* packed, float* y, int M, int K, int N,
+                                   void* workspace, size_t workspace_bytes, void* stream);
+int    laplace_cuda_mxfp4_moe_grouped_dev(const float* x, int x_rows, const uint8_t* packed, const int* pair_expert,
+                                          const int* pair_row, int n_pairs, int n_experts_total, float* y, int K, int N,
+                                          void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- row-split prefill: the GEMM stores into every GPU's buffer --------------------------
  * laplace_cuda_gemm_peers_dev is laplace_cuda_gemm_dev for M > 8 over a weight matrix split along N: this GPU's

@@ -45,6 +45,12 @@ SYMBOLS = {
     "laplace_cuda_dequantize_dev": (_i, [_vp, _u32, _vp, C.c_longlong, _vp]),
     "laplace_cuda_embed_rows_dev": (_i, [_vp, _u32, _vp, _i, _i, C.c_longlong, C.c_float, _vp, _vp]),
     "laplace_cuda_lm_head_dev": (_i, [_vp, _vp, _u32, _vp, _i, _i, _i, C.c_float, _vp]),
+    "laplace_cuda_mxfp4_quantize_dev": (_i, [_vp, _u32, _vp, C.c_longlong, _vp]),
+    "laplace_cuda_mxfp4_packed_size": (_sz, [_i, _i, _i]),
+    "laplace_cuda_mxfp4_pack_dev": (_i, [_vp, _vp, _i, _i, _i, _vp]),
+    "laplace_cuda_mxfp4_workspace_size": (_sz, [_i, _i, _i, _i]),
+    "laplace_cuda_mxfp4_gemm_dev": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp, _sz, _vp]),
+    "laplace_cuda_mxfp4_moe_grouped_dev": (_i, [_vp, _i, _vp, _vp, _vp, _i, _i, _vp, _i, _i, _vp, _sz, _vp]),
     "laplace_cuda_gguf_open": (_i, [C.c_char_p, _i, _i, C.POINTER(C.c_char_p), _i, C.POINTER(_vp)]),
     "laplace_cuda_gguf_upload": (_i, [_vp]),
     "laplace_cuda_gguf_tensor_count": (_i, [_vp]),

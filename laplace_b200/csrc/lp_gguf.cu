@@ -59,6 +59,7 @@ TypeGeo type_geo(uint32_t t) {
         case 27: return {1, 8};       // I64
         case 28: return {1, 8};       // F64
         case 30: return {1, 2};       // BF16
+        case 39: return {32, 17};     // MXFP4, which Laplace's table does not know
         default: return {0, 0};
     }
 }

@@ -1,0 +1,453 @@
+// lp_mx.cu - MXFP4 weights (GGUF type 39): quantizer, the layout in HBM that the products read, and the products with
+// MXFP8 activations - one matrix, or experts with ragged numbers of rows. No reference counterpart (Laplace has no such type).
+//
+// Formats. Blocks of 32 values of a row share a power of two 2^s, held as s + 127 in one byte (255: the block is NaN).
+//   MXFP4  e2m1 values 0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives. GGUF block, 17 bytes: s + 127, then 16 bytes, value l in the low,
+//          value l + 16 in the high half of byte l. Quantizer: s = floor(log2(amax)) - 2, nearest, ties to even, magnitudes over 6 held as 6.
+//   MXFP8  e4m3 values up to 448, for activations: the smallest s with amax <= 448 * 2^s, so that no value is cut off (with
+//          floor(log2(amax)) - 8 a fifth of the blocks would lose up to an eighth of their largest value).
+// Scaling by a power of two is exact and the roundings are the hardware's, so the quantized values are the definition's to the bit.
+//
+// Packed weights. A matrix of N rows of K values is cut into tiles of 128 rows x 128 values; rows and values behind the end are 0.
+//   q   [matrix][row tile][k tile][128 rows][64 bytes]    value 2 i in the low, 2 i + 1 in the high half of byte i
+//   sf  [matrix][row tile][k tile][512 bytes]             behind all q: the scale byte of (row r, 32-value block b of the four) at
+//                                                         (r % 32) * 16 + (r / 32) * 4 + b, the order in which the tensor core takes them
+// A tile is 8 KB in one piece (rows apart would be read 64 bytes at a time), 0.53 bytes per value as in the file.
+// Quantized activations (workspace): image [k tile][row][128 bytes], 16-byte pieces of a row swizzled by row % 8 as the tensor core
+// reads them, and the scales [k tile][128-row group][512 bytes] in the order above.
+#include <cuda_bf16.h>
+
+#include "lp_mx.cuh"
+
+namespace lp {
+namespace {
+
+using namespace mx;
+
+// ---- values -> GGUF blocks ---------------------------------------------------------------------------------------
+template <class T> __device__ __forceinline__ void load8(const T* p, float (&v)[8]);
+template <> __device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+template <> __device__ __forceinline__ void load8<__half>(const __half* p, float (&v)[8]) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        v[2 * i] = f.x; v[2 * i + 1] = f.y;
+    }
+}
+template <> __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&v)[8]) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+}
+__device__ __forceinline__ float amax8(const float (&v)[8]) {
+    float a = fabsf(v[0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) a = max_nan(a, fabsf(v[i]));
+    return a;
+}
+// 2^e for e in [-127, 127]
+__device__ __forceinline__ float pow2(int e) { return e == -127 ? __uint_as_float(0x00400000u) : __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+
+// A block per 4 lanes, 8 values each; 64 blocks a CTA, gathered in shared memory and written in order.
+constexpr int QB = 64;
+template <class T>
+__global__ void __launch_bounds__(256) mxfp4_quantize_kernel(const T* __restrict__ x, uint8_t* __restrict__ w, long long n_blocks) {
+    __shared__ __align__(16) uint8_t out[QB * 17];
+    const int blk = threadIdx.x >> 2, part = threadIdx.x & 3;
+    const long long b0 = static_cast<long long>(blockIdx.x) * QB;
+    const int here = n_blocks - b0 < QB ? static_cast<int>(n_blocks - b0) : QB;
+    float v[8] = {};
+    if (blk < here) load8(x + (b0 + blk) * 32 + part * 8, v);
+    float a = amax8(v);
+    a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 1));
+    a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 2));
+    const bool bad = !(a < __uint_as_float(0x7f800000u));            // infinity or NaN: the block stands for NaN
+    int s = static_cast<int>(__float_as_uint(a) >> 23) - 129;         // floor(log2(a)) - 2; 0 and numbers below the normal ones: the lowest
+    if (s < -127) s = -127;
+    const float inv = pow2(-s);
+    uint32_t c = 0;                                                   // eight codes, value i in bits 4 i
+    if (!bad) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c |= e2m1x2(v[2 * i] * inv, v[2 * i + 1] * inv) << (8 * i);
+    }
+    const uint32_t o = __shfl_xor_sync(0xffffffffu, c, 2);            // lanes 0 and 1 hold values 0..15, lanes 2 and 3 16..31
+    if (part < 2) {
+        uint8_t* d = out + blk * 17 + 1 + part * 8;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d[i] = static_cast<uint8_t>(((c >> (4 * i)) & 15u) | (((o >> (4 * i)) & 15u) << 4));
+        if (part == 0) out[blk * 17] = static_cast<uint8_t>(bad ? 255 : s + 127);
+    }
+    __syncthreads();
+    uint8_t* dst = w + b0 * 17;
+    const int bytes = here * 17;
+    if ((reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+        for (int i = threadIdx.x; i < bytes / 16; i += 256) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(out)[i];
+        for (int i = (bytes & ~15) + threadIdx.x; i < bytes; i += 256) dst[i] = out[i];
+    } else {
+        for (int i = threadIdx.x; i < bytes; i += 256) dst[i] = out[i];
+    }
+}
+
+// ---- GGUF blocks -> packed tiles -----------------------------------------------------------------------------------
+// A thread per block: rows of a tile x its four blocks. Blocks start at any byte: 17 bytes lie in five aligned words, whose bytes
+// outside the block share a word with it.
+__global__ void __launch_bounds__(512) mxfp4_pack_kernel(const uint8_t* __restrict__ w, uint8_t* __restrict__ q, uint8_t* __restrict__ sf, int N, int K, int rts, int kts) {
+    const int kt = blockIdx.x, rt = blockIdx.y % rts, e = blockIdx.y / rts;
+    const int r = threadIdx.x >> 2, b = threadIdx.x & 3;
+    const int row = rt * 128 + r, k32 = kt * 4 + b, bpr = K / 32;
+    uint4 o = make_uint4(0, 0, 0, 0);
+    uint8_t scale = 127;
+    if (row < N && k32 < bpr) {
+        const uint8_t* p = w + ((static_cast<size_t>(e) * N + row) * bpr + k32) * 17;
+        const uint32_t* a = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(p) & ~static_cast<uintptr_t>(3));
+        const uint32_t sh = (reinterpret_cast<uintptr_t>(p) & 3) * 8;
+        const uint32_t x0 = __ldg(a), x1 = __ldg(a + 1), x2 = __ldg(a + 2), x3 = __ldg(a + 3), x4 = __ldg(a + 4);
+        const uint32_t y0 = __funnelshift_r(x0, x1, sh), y1 = __funnelshift_r(x1, x2, sh), y2 = __funnelshift_r(x2, x3, sh), y3 = __funnelshift_r(x3, x4, sh),
+                       y4 = x4 >> sh;
+        scale = static_cast<uint8_t>(y0);
+        const uint32_t in[4] = {__funnelshift_r(y0, y1, 8), __funnelshift_r(y1, y2, 8), __funnelshift_r(y2, y3, 8), __funnelshift_r(y3, y4, 8)};
+        uint32_t lo[4], hi[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t l = in[i] & 0x0f0f0f0fu, h = (in[i] >> 4) & 0x0f0f0f0fu;
+            lo[i] = l | (l >> 4);                 // bytes 0 and 2: two neighbours each
+            hi[i] = h | (h >> 4);
+        }
+        o = make_uint4(__byte_perm(lo[0], lo[1], 0x6420), __byte_perm(lo[2], lo[3], 0x6420), __byte_perm(hi[0], hi[1], 0x6420), __byte_perm(hi[2], hi[3], 0x6420));
+    }
+    const size_t tile = (static_cast<size_t>(e) * rts + rt) * kts + kt;
+    *reinterpret_cast<uint4*>(q + tile * Q_TILE + r * 64 + b * 16) = o;
+    sf[tile * SF_TILE + (r & 31) * 16 + (r >> 5) * 4 + b] = scale;
+}
+
+// ---- fp32 rows -> MXFP8 image -------------------------------------------------------------------------------------
+// A warp takes 256 values of a row: a 32-value block per 4 lanes. GROUPED: the row of x and the place in the image by pair.
+template <bool GROUPED>
+__global__ void __launch_bounds__(256) mx_act_kernel(const float* __restrict__ x, int K, int kts, int rows, ActDst d, const int* __restrict__ pair_row, const int* __restrict__ dst_row,
+                                                     unsigned* __restrict__ counters, int n_counters) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int lane = threadIdx.x & 31, segs = (kts + 1) >> 1;
+    const long long id = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < n_counters; i += 256) counters[i] = 0;
+    const int row = static_cast<int>(id / segs), seg = static_cast<int>(id % segs);
+    if (row >= rows) return;
+    int src = row, dst = row;
+    if (GROUPED) {
+        dst = dst_row[row];
+        if (dst < 0) return;
+        if (pair_row) src = pair_row[row];
+    }
+    const int k = seg * 256 + lane * 8;
+    float v[8] = {};
+    if (k < K) load8(x + static_cast<size_t>(src) * K + k, v);         // K is a multiple of 32: all eight or none
+    float a = amax8(v);
+    a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 1));
+    a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 2));
+    const bool bad = !(a < __uint_as_float(0x7f800000u));
+    const uint32_t bits = __float_as_uint(a);
+    int s = static_cast<int>(bits >> 23) - 135 + ((bits & 0x7fffffu) > 0x600000u);      // a = m 2^e, 1 <= m < 2: e - 8 up to m = 1.75, else e - 7
+    if (s < -127) s = -127;
+    const float inv = pow2(-s);
+    uint2 q;
+    q.x = bad ? 0x7f7f7f7fu : e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+    q.y = bad ? 0x7f7f7f7fu : e4m3x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+    uint32_t sc = (bad ? 255u : static_cast<uint32_t>(s + 127)) << (8 * ((lane >> 2) & 3));
+    sc |= __shfl_xor_sync(0xffffffffu, sc, 4);
+    sc |= __shfl_xor_sync(0xffffffffu, sc, 8);
+    const int kt = seg * 2 + (lane >> 4);
+    if (kt >= kts) return;
+    const int piece = (lane & 15) >> 1;
+    *reinterpret_cast<uint2*>(d.img + (static_cast<size_t>(kt) * d.rows + dst) * 128 + ((piece ^ (dst & 7)) << 4) + (lane & 1) * 8) = q;
+    if ((lane & 15) == 0)
+        *reinterpret_cast<uint32_t*>(d.sf + (static_cast<size_t>(kt) * d.groups + (dst >> 7)) * SF_TILE + (dst & 31) * 16 + ((dst >> 5) & 3) * 4) = sc;
+}
+
+// ---- pairs -> places in the image and a table of token tiles --------------------------------------------------------
+// Every block counts all pairs by expert and gives each expert its rows of the image, 32 at a time (a scale byte's place is by row % 32);
+// its warps then walk the pairs of one expert each, in order, so that a pair's place does not depend on timing.
+__global__ void __launch_bounds__(1024) mx_group_kernel(const int* __restrict__ pair_expert, const int* __restrict__ pair_row, int P, int E, int x_rows, int tile_w,
+                                                        int* __restrict__ dst_row, int* __restrict__ out_row, int4* __restrict__ tab, int* __restrict__ n_tiles, int* err) {
+    extern __shared__ int sm[];
+    int* count = sm;
+    int* start = sm + E;           // [E + 1]
+    int* tile0 = sm + 2 * E + 1;   // [E + 1]
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    for (int i = threadIdx.x; i < E; i += blockDim.x) count[i] = 0;
+    __syncthreads();
+    auto expert_of = [&](int p) {
+        const int e = __ldg(pair_expert + p);
+        if (e < 0) return -1;
+        if (e >= E || (pair_row && static_cast<unsigned>(__ldg(pair_row + p)) >= static_cast<unsigned>(x_rows))) return -2;
+        return e;
+    };
+    for (int p = threadIdx.x; p < P; p += blockDim.x) {
+        const int e = expert_of(p);
+        if (e >= 0) atomicAdd(count + e, 1);
+        else if (blockIdx.x == 0) {
+            dst_row[p] = -1;
+            if (e == -2) atomicCAS(err, DEV_OK, DEV_BAD_INDEX);
+        }
+    }
+    __syncthreads();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (warp == 0) {
+        int rows = 0, tiles = 0;
+        for (int e0 = 0; e0 < E; e0 += 32) {
+            const int c = e0 + lane < E ? count[e0 + lane] : 0;
+            int r = (c + 31) & ~31, t = (c + tile_w - 1) / tile_w;
+            int ri = r, ti = t;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int a = __shfl_up_sync(0xffffffffu, ri, o), b = __shfl_up_sync(0xffffffffu, ti, o);
+                if (lane >= o) { ri += a; ti += b; }
+            }
+            if (e0 + lane < E) { start[e0 + lane] = rows + ri - r; tile0[e0 + lane] = tiles + ti - t; }
+            rows += __shfl_sync(0xffffffffu, ri, 31);
+            tiles += __shfl_sync(0xffffffffu, ti, 31);
+        }
+        if (lane == 0 && blockIdx.x == 0) *n_tiles = tiles;
+    }
+    __syncthreads();
+    for (int e = blockIdx.x * 32 + warp; e < E; e += gridDim.x * 32) {
+        const int c = count[e], s = start[e];
+        if (!c) continue;
+        for (int t = lane; t * tile_w < c; t += 32) tab[tile0[e] + t] = make_int4(e, s + t * tile_w, min(tile_w, c - t * tile_w), 0);
+        int at = s;
+        for (int p0 = 0; p0 < P; p0 += 32) {
+            const int p = p0 + lane;
+            const bool mine = p < P && expert_of(p) == e;
+            const unsigned m = __ballot_sync(0xffffffffu, mine);
+            if (mine) {
+                const int r = at + __popc(m & ((1u << lane) - 1));
+                dst_row[p] = r;
+                out_row[r] = p;
+            }
+            at += __popc(m);
+        }
+    }
+}
+
+// ---- the product, simplest form: a thread per weight row, 8 tokens at a time -----------------------------------------
+__device__ __forceinline__ float e2m1_value(uint32_t c) {
+    const float t[8] = {0.f, .5f, 1.f, 1.5f, 2.f, 3.f, 4.f, 6.f};
+    const float m = t[c & 7];
+    return c & 8 ? -m : m;
+}
+template <bool GROUPED>
+__global__ void __launch_bounds__(128) mx_plain_kernel(MxArgs a) {
+    __shared__ float xs[8][128];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int r = threadIdx.x, per_tile = (a.tile_w + 7) / 8;
+    const long long jobs = GROUPED ? static_cast<long long>(*a.n_tiles) * per_tile * a.rts : static_cast<long long>((a.M + 7) / 8) * a.rts;
+    for (long long j = blockIdx.x; j < jobs; j += gridDim.x) {
+        const int rt = static_cast<int>(j % a.rts);
+        int row0, n, e = 0;
+        if (GROUPED) {
+            const int4 t = a.tab[j / a.rts / per_tile];
+            const int off = static_cast<int>(j / a.rts % per_tile) * 8;
+            e = t.x; row0 = t.y + off; n = min(8, t.z - off);
+            if (n <= 0) continue;
+        } else {
+            row0 = static_cast<int>(j / a.rts) * 8;
+            n = min(8, a.M - row0);
+        }
+        float acc[8] = {};
+        for (int kt = 0; kt < a.kts; ++kt) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < n * 128; i += 128) {
+                const int row = row0 + (i >> 7), c = i & 127;
+                const uint8_t q = a.img[(static_cast<size_t>(kt) * a.img_rows + row) * 128 + (((c >> 4) ^ (row & 7)) << 4) + (c & 15)];
+                const uint8_t s = a.sfb[(static_cast<size_t>(kt) * a.groups + (row >> 7)) * SF_TILE + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (c >> 5)];
+                const float f = e4m3_value(q);
+                xs[i >> 7][c] = s == 255 ? __uint_as_float(0x7fc00000u) : f * pow2(static_cast<int>(s) - 127);
+            }
+            __syncthreads();
+            const size_t tile = (static_cast<size_t>(e) * a.rts + rt) * a.kts + kt;
+            for (int b = 0; b < 4; ++b) {
+                const uint4 q = *reinterpret_cast<const uint4*>(a.q + tile * Q_TILE + r * 64 + b * 16);
+                const uint8_t s = a.sfa[tile * SF_TILE + (r & 31) * 16 + (r >> 5) * 4 + b];
+                const float sc = s == 255 ? __uint_as_float(0x7fc00000u) : pow2(static_cast<int>(s) - 127);
+                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+                for (int i = 0; i < 32; ++i) {
+                    const float v = e2m1_value(w[i >> 3] >> (4 * (i & 7))) * sc;
+                    for (int m = 0; m < n; ++m) acc[m] = fmaf(v, xs[m][b * 32 + i], acc[m]);
+                }
+            }
+        }
+        const int col = rt * 128 + r;
+        if (col < a.N)
+            for (int m = 0; m < n; ++m) a.y[static_cast<size_t>(GROUPED ? a.out_row[row0 + m] : row0 + m) * a.N + col] = acc[m];
+    }
+}
+
+size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
+
+// What a call keeps in its workspace, and where.
+struct Plan {
+    int    kts, rts, img_rows, groups, tile_w, max_tiles, n_counters;
+    size_t img, sf, counters, dst_row, out_row, tab, n_tiles, bytes;
+};
+Plan plan_of(int rows, int experts, int K, int N) {
+    Plan p{};
+    p.kts = (K + 127) / 128;
+    p.rts = (N + 127) / 128;
+    const long long most = experts ? rows + 31ll * (experts < rows ? experts : rows) : rows;
+    p.img_rows = static_cast<int>((most + 7) & ~7ll);
+    p.groups = (p.img_rows + 127) / 128;
+    p.tile_w = 32;
+    p.max_tiles = experts ? rows / p.tile_w + (experts < rows ? experts : rows) : 0;
+    size_t at = 0;
+    auto take = [&](size_t n) { const size_t here = at; at += align256(n); return here; };
+    p.img = take(static_cast<size_t>(p.kts) * p.img_rows * 128);
+    p.sf = take(static_cast<size_t>(p.kts) * p.groups * SF_TILE);
+    p.counters = take(p.n_counters * sizeof(unsigned));
+    if (experts) {
+        p.dst_row = take(static_cast<size_t>(rows) * 4);
+        p.out_row = take(static_cast<size_t>(p.img_rows) * 4);
+        p.tab = take(static_cast<size_t>(p.max_tiles) * sizeof(int4));
+        p.n_tiles = take(4);
+    }
+    p.bytes = at;
+    return p;
+}
+
+template <bool GROUPED>
+int launch_product(const float* x, int x_rows, const uint8_t* packed, const int* pair_expert, const int* pair_row, int rows, int experts, float* y, int K, int N,
+                   uint8_t* ws, cudaStream_t st) {
+    const Plan p = plan_of(rows, GROUPED ? experts : 0, K, N);
+    Context& c = ctx();
+    MxArgs a{};
+    a.q = packed;
+    a.sfa = packed + static_cast<size_t>(GROUPED ? experts : 1) * p.rts * p.kts * Q_TILE;
+    a.img = ws + p.img; a.sfb = ws + p.sf; a.y = y;
+    a.M = rows; a.N = N; a.kts = p.kts; a.rts = p.rts; a.img_rows = p.img_rows; a.groups = p.groups; a.tile_w = p.tile_w;
+    int* dst_row = nullptr;
+    int rc;
+    if (GROUPED) {
+        dst_row = reinterpret_cast<int*>(ws + p.dst_row);
+        a.out_row = reinterpret_cast<int*>(ws + p.out_row);
+        a.tab = reinterpret_cast<int4*>(ws + p.tab);
+        a.n_tiles = reinterpret_cast<int*>(ws + p.n_tiles);
+        rc = launch_early(mx_group_kernel, dim3((experts + 31) / 32), 1024, (3 * static_cast<size_t>(experts) + 2) * sizeof(int), st, pair_expert, pair_row, rows, experts, x_rows, p.tile_w,
+                          dst_row, reinterpret_cast<int*>(ws + p.out_row), reinterpret_cast<int4*>(ws + p.tab), reinterpret_cast<int*>(ws + p.n_tiles), c.d_err);
+        c.launches++;
+        if (rc) return rc;
+    }
+    const long long warps = static_cast<long long>(rows) * ((p.kts + 1) / 2);
+    rc = launch_early(mx_act_kernel<GROUPED>, dim3(static_cast<unsigned>((warps + 7) / 8)), 256, 0, st, x, K, p.kts, rows, ActDst{ws + p.img, ws + p.sf, p.img_rows, p.groups},
+                      pair_row, static_cast<const int*>(dst_row), reinterpret_cast<unsigned*>(ws + p.counters), p.n_counters);
+    c.launches++;
+    if (rc) return rc;
+    rc = launch_early(mx_plain_kernel<GROUPED>, dim3(c.sm_count * 8), 128, 0, st, a);
+    c.launches++;
+    return rc;
+}
+
+int bad_shape(const char* what, int K, int N, long long experts) {
+    if (K <= 0 || N <= 0 || experts <= 0 || K % 32) return fail(LAPLACE_ERR_ARG, "%s: K=%d (a positive multiple of 32) N=%d experts=%lld", what, K, N, experts);
+    // rows of 64 bytes that the tensor map of the weights counts
+    if (experts * ((N + 127ll) / 128) * ((K + 127) / 128) * 128 > 0x7fffffffll) return fail(LAPLACE_ERR_LIMIT, "%s: %lld x %d x %d values are more than one call takes", what, experts, N, K);
+    return LAPLACE_OK;
+}
+bool misaligned(const void* p, unsigned n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }
+constexpr int MAX_EXPERTS = 4000;      // three counters each in 48 KB of shared memory
+
+}  // namespace
+
+int launch_mxfp4_dequantize(const uint8_t* w, float* dst, long long n, float scale, cudaStream_t st);
+
+}  // namespace lp
+
+using namespace lp;
+
+extern "C" {
+
+#define MX_READY() if (!ctx().ready) return fail(LAPLACE_ERR_STATE, "laplace_cuda_init has not been called (or found no GPU)")
+#define MX_STREAM(s) ((s) ? static_cast<cudaStream_t>(s) : ctx().stream)
+
+int laplace_cuda_mxfp4_quantize_dev(const void* x, uint32_t x_type, uint8_t* w, long long n, void* stream) {
+    MX_READY();
+    if (x_type != 0 && x_type != 1 && x_type != 30) return LAPLACE_UNSUPPORTED;
+    if (n == 0) return LAPLACE_OK;
+    if (!x || !w || n < 0 || n % 32) return fail(LAPLACE_ERR_ARG, "mxfp4_quantize: n=%lld is not a multiple of 32, or a null pointer", n);
+    if (misaligned(x, 16)) return fail(LAPLACE_ERR_ARG, "mxfp4_quantize: x must be 16-byte aligned");
+    const long long blocks = n / 32, grid = (blocks + QB - 1) / QB;
+    if (grid > 0x7fffffffll) return fail(LAPLACE_ERR_LIMIT, "mxfp4_quantize: n=%lld", n);
+    cudaStream_t st = MX_STREAM(stream);
+    const unsigned g = static_cast<unsigned>(grid);
+    if (x_type == 0) mxfp4_quantize_kernel<<<g, 256, 0, st>>>(static_cast<const float*>(x), w, blocks);
+    else if (x_type == 1) mxfp4_quantize_kernel<<<g, 256, 0, st>>>(static_cast<const __half*>(x), w, blocks);
+    else mxfp4_quantize_kernel<<<g, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(x), w, blocks);
+    ctx().launches++;
+    return cuda_check(cudaGetLastError(), "mxfp4_quantize launch");
+}
+
+size_t laplace_cuda_mxfp4_packed_size(int n_experts, int N, int K) {
+    if (n_experts <= 0 || N <= 0 || K <= 0 || K % 32) return 0;
+    return static_cast<size_t>(n_experts) * ((N + 127) / 128) * ((K + 127) / 128) * (Q_TILE + SF_TILE);
+}
+
+int laplace_cuda_mxfp4_pack_dev(const uint8_t* w, uint8_t* packed, int n_experts, int N, int K, void* stream) {
+    MX_READY();
+    if (const int rc = bad_shape("mxfp4_pack", K, N, n_experts)) return rc;
+    if (!w || !packed || misaligned(packed, 128)) return fail(LAPLACE_ERR_ARG, "mxfp4_pack: null pointer, or packed is not 128-byte aligned");
+    const int rts = (N + 127) / 128, kts = (K + 127) / 128;
+    // row tiles on the grid's second axis, 65535 a launch: whole experts at a time, or (one expert with more tiles) refused
+    if (rts > 65535) return fail(LAPLACE_ERR_LIMIT, "mxfp4_pack: N=%d", N);
+    const int step = 65535 / rts;
+    const size_t n_tiles = static_cast<size_t>(n_experts) * rts * kts;
+    for (int e = 0; e < n_experts; e += step) {
+        const int here = n_experts - e < step ? n_experts - e : step;
+        const size_t t0 = static_cast<size_t>(e) * rts * kts;
+        mxfp4_pack_kernel<<<dim3(kts, rts * here), 512, 0, MX_STREAM(stream)>>>(w + static_cast<size_t>(e) * N * (K / 32) * 17, packed + t0 * Q_TILE,
+                                                                                packed + n_tiles * Q_TILE + t0 * SF_TILE, N, K, rts, kts);
+        ctx().launches++;
+    }
+    return cuda_check(cudaGetLastError(), "mxfp4_pack launch");
+}
+
+size_t laplace_cuda_mxfp4_workspace_size(int rows, int n_experts, int K, int N) {
+    if (rows <= 0 || n_experts < 0 || K <= 0 || N <= 0 || K % 32) return 0;
+    return plan_of(rows, n_experts, K, N).bytes;
+}
+
+int laplace_cuda_mxfp4_gemm_dev(const float* x, const uint8_t* packed, float* y, int M, int K, int N, void* workspace, size_t workspace_bytes, void* stream) {
+    MX_READY();
+    if (const int rc = bad_shape("mxfp4_gemm", K, N, 1)) return rc;
+    if (M < 0) return fail(LAPLACE_ERR_ARG, "mxfp4_gemm: M=%d", M);
+    if (M == 0) return LAPLACE_OK;
+    if (M > 1 << 24) return fail(LAPLACE_ERR_LIMIT, "mxfp4_gemm: M=%d", M);
+    if (!x || !packed || !y || !workspace) return fail(LAPLACE_ERR_ARG, "mxfp4_gemm: null pointer");
+    if (misaligned(x, 16) || misaligned(packed, 128) || misaligned(workspace, 256) || misaligned(y, 4))
+        return fail(LAPLACE_ERR_ARG, "mxfp4_gemm: x must be 16-byte, packed 128-byte, workspace 256-byte aligned");
+    if (workspace_bytes < plan_of(M, 0, K, N).bytes) return fail(LAPLACE_ERR_ARG, "mxfp4_gemm: workspace of %zu bytes, %zu needed", workspace_bytes, plan_of(M, 0, K, N).bytes);
+    return launch_product<false>(x, M, packed, nullptr, nullptr, M, 1, y, K, N, static_cast<uint8_t*>(workspace), MX_STREAM(stream));
+}
+
+int laplace_cuda_mxfp4_moe_grouped_dev(const float* x, int x_rows, const uint8_t* packed, const int* pair_expert, const int* pair_row, int n_pairs, int n_experts_total, float* y,
+                                       int K, int N, void* workspace, size_t workspace_bytes, void* stream) {
+    MX_READY();
+    if (const int rc = bad_shape("mxfp4_moe_grouped", K, N, n_experts_total)) return rc;
+    if (n_pairs < 0 || x_rows < 0) return fail(LAPLACE_ERR_ARG, "mxfp4_moe_grouped: n_pairs=%d x_rows=%d", n_pairs, x_rows);
+    if (n_pairs == 0) return LAPLACE_OK;
+    if (n_pairs > 1 << 24) return fail(LAPLACE_ERR_LIMIT, "mxfp4_moe_grouped: n_pairs=%d", n_pairs);
+    if (n_experts_total > MAX_EXPERTS) return fail(LAPLACE_ERR_LIMIT, "mxfp4_moe_grouped: %d experts, %d at most", n_experts_total, MAX_EXPERTS);
+    if (!x || !packed || !pair_expert || !y || !workspace) return fail(LAPLACE_ERR_ARG, "mxfp4_moe_grouped: null pointer");
+    if (!pair_row && x_rows < n_pairs) return fail(LAPLACE_ERR_ARG, "mxfp4_moe_grouped: %d rows of x for %d pairs", x_rows, n_pairs);
+    if (misaligned(x, 16) || misaligned(packed, 128) || misaligned(workspace, 256) || misaligned(y, 4) || misaligned(pair_expert, 4) || misaligned(pair_row, 4))
+        return fail(LAPLACE_ERR_ARG, "mxfp4_moe_grouped: x must be 16-byte, packed 128-byte, workspace 256-byte aligned");
+    const size_t need = plan_of(n_pairs, n_experts_total, K, N).bytes;
+    if (workspace_bytes < need) return fail(LAPLACE_ERR_ARG, "mxfp4_moe_grouped: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    return launch_product<true>(x, x_rows, packed, pair_expert, pair_row, n_pairs, n_experts_total, y, K, N, static_cast<uint8_t*>(workspace), MX_STREAM(stream));
+}
+
+}  // extern "C"

@@ -23,7 +23,7 @@ namespace lp {
 namespace {
 
 constexpr uint32_t T_F32 = 0, T_F16 = 1, T_Q4_0 = 2, T_Q5_0 = 6, T_Q8_0 = 8, T_Q2_K = 10, T_Q3_K = 11, T_Q4_K = 12,
-                   T_Q5_K = 13, T_Q6_K = 14, T_BF16 = 30;
+                   T_Q5_K = 13, T_Q6_K = 14, T_BF16 = 30, T_MXFP4 = 39;
 
 struct Geo { int elems, bytes; };       // per block; plain types are handled as "blocks" of 16 values
 __host__ __device__ constexpr Geo geo_of(uint32_t t) {
@@ -38,6 +38,7 @@ __host__ __device__ constexpr Geo geo_of(uint32_t t) {
         case T_Q4_K: return {256, 144};
         case T_Q5_K: return {256, 176};
         case T_Q6_K: return {256, 210};
+        case T_MXFP4: return {32, 17};
         default: return {0, 0};
     }
 }
@@ -168,6 +169,19 @@ __device__ __forceinline__ void decode16(uint32_t type, const uint8_t* __restric
                 const int nib = (qtr & 2) ? (ql[l] >> 4) : (ql[l] & 0xF);
                 const int q = nib | (((qh[l] >> (2 * qtr)) & 3) << 4);
                 v[l] = __fmul_rn(ds, static_cast<float>(q - 32));
+            }
+            break;
+        }
+        case T_MXFP4: {
+            // scale byte s + 127 (255: NaN), qs[16]: value = 2^s * e2m1
+            const uint32_t e = b[0];
+            const float d = __uint_as_float(e == 255 ? 0x7fc00000u : e ? e << 23 : 0x00400000u);
+#pragma unroll
+            for (int l = 0; l < 16; ++l) {
+                const uint32_t c = g ? (b[1 + l] >> 4) : (b[1 + l] & 0xF);
+                const uint32_t m = c & 7;          // 0 and 0.5, else 1 or 1.5 times 2^(m / 2 - 1)
+                const float a = m < 2 ? 0.5f * static_cast<float>(m) : __uint_as_float(((126 + (m >> 1)) << 23) | ((m & 1) << 22));
+                v[l] = __fmul_rn(d, c & 8 ? -a : a);
             }
             break;
         }
@@ -540,6 +554,8 @@ cudaError_t launch_f32act(const float* x, const uint8_t* w, uint32_t type, float
 bool f32act_type(uint32_t type) {
     return type == T_F32 || type == T_F16 || type == T_BF16 || type == T_Q2_K || type == T_Q3_K || type == T_Q5_K;
 }
+// MXFP4 blocks are 17 bytes and read by the byte
+static uintptr_t align_mask(uint32_t type) { return type == T_F32 ? 15 : type == T_MXFP4 ? 0 : 1; }
 bool dequant_type(uint32_t type) { return geo_of(type).elems != 0; }
 size_t any_row_bytes(uint32_t type, long long K) {
     const Geo g = geo_of(type);
@@ -587,8 +603,8 @@ int launch_dequantize(const uint8_t* w, uint32_t type, float* dst, long long n, 
     const Geo g = geo_of(type);
     if (!g.elems) return LAPLACE_UNSUPPORTED;
     if (!w || !dst || n <= 0 || n % g.elems) return fail(LAPLACE_ERR_ARG, "dequantize: n=%lld is not a positive multiple of %d", n, g.elems);
-    if ((reinterpret_cast<uintptr_t>(dst) & 15) || (reinterpret_cast<uintptr_t>(w) & (type == T_F32 ? 15 : 1)))
-        return fail(LAPLACE_ERR_ARG, "dequantize: dst must be 16-byte aligned, blocks 2-byte (F32: 16-byte) aligned");
+    if ((reinterpret_cast<uintptr_t>(dst) & 15) || (reinterpret_cast<uintptr_t>(w) & align_mask(type)))
+        return fail(LAPLACE_ERR_ARG, "dequantize: dst must be 16-byte aligned, blocks 2-byte (F32: 16-byte, MXFP4: any) aligned");
     const long long groups = n / 16;
     long long blocks = (groups + 255) / 256;
     if (blocks > static_cast<long long>(ctx().sm_count) * 16) blocks = static_cast<long long>(ctx().sm_count) * 16;
@@ -603,8 +619,8 @@ int launch_embed_rows(const uint8_t* w, uint32_t type, const int* tokens, int M,
     if (!g.elems) return LAPLACE_UNSUPPORTED;
     if (!w || !tokens || !dst || M <= 0 || H <= 0 || H % g.elems || vocab <= 0)
         return fail(LAPLACE_ERR_ARG, "embed_rows: M=%d H=%d (a multiple of %d expected) vocab=%lld", M, H, g.elems, vocab);
-    if ((reinterpret_cast<uintptr_t>(dst) & 15) || (reinterpret_cast<uintptr_t>(w) & (type == T_F32 ? 15 : 1)))
-        return fail(LAPLACE_ERR_ARG, "embed_rows: dst must be 16-byte aligned, blocks 2-byte (F32: 16-byte) aligned");
+    if ((reinterpret_cast<uintptr_t>(dst) & 15) || (reinterpret_cast<uintptr_t>(w) & align_mask(type)))
+        return fail(LAPLACE_ERR_ARG, "embed_rows: dst must be 16-byte aligned, blocks 2-byte (F32: 16-byte, MXFP4: any) aligned");
     embed_rows_kernel<<<M, 256, 0, st>>>(w, type, tokens, H, vocab, scale, dst, ctx().d_err);
     ctx().launches++;
     return cuda_check(cudaGetLastError(), "embed_rows launch");

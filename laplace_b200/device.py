@@ -248,6 +248,68 @@ def lm_head(x: torch.Tensor, w: torch.Tensor, t: int, M: int, K: int, N: int, so
     return y
 
 
+_MX_FLOATS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
+
+
+def _here(*tensors) -> bool:
+    return all(t.is_cuda and t.is_contiguous() and t.device.index == torch.cuda.current_device() for t in tensors if t is not None)
+
+
+def mxfp4_quantize(x: torch.Tensor, w: torch.Tensor | None = None) -> torch.Tensor:
+    """Values (fp32, fp16 or bf16; rows a multiple of 32 long) -> MXFP4 blocks as GGUF holds them, flat bytes
+    (laplace_cuda_mxfp4_quantize_dev). dequantize, embed_rows and mxfp4_pack take them."""
+    L = lib()
+    assert x.dtype in _MX_FLOATS and _here(x, w) and x.dim() >= 1 and x.shape[-1] % 32 == 0
+    n = x.numel()
+    if w is None:
+        w = torch.empty(n // 32 * 17, dtype=torch.uint8, device=x.device)
+    assert w.dtype == torch.uint8 and w.numel() >= n // 32 * 17
+    _check(L, L.laplace_cuda_mxfp4_quantize_dev(x.data_ptr(), _MX_FLOATS[x.dtype], w.data_ptr(), n, _stream()))
+    return w
+
+
+def mxfp4_pack(w: torch.Tensor, N: int, K: int, n_experts: int = 1) -> torch.Tensor:
+    """GGUF MXFP4 blocks of n_experts matrices [N][K] -> the layout that mxfp4_gemm and mxfp4_moe_grouped read
+    (laplace_cuda_mxfp4_pack_dev): once, when the weights are loaded."""
+    L = lib()
+    assert w.dtype == torch.uint8 and _here(w) and w.numel() >= n_experts * N * any_row_bytes(39, K)
+    packed = torch.empty(L.laplace_cuda_mxfp4_packed_size(n_experts, N, K), dtype=torch.uint8, device=w.device)
+    _check(L, L.laplace_cuda_mxfp4_pack_dev(w.data_ptr(), packed.data_ptr(), n_experts, N, K, _stream()))
+    return packed
+
+
+def mxfp4_gemm(x: torch.Tensor, packed: torch.Tensor, M: int, K: int, N: int, y: torch.Tensor | None = None) -> torch.Tensor:
+    """y[m] = W . x[m] with packed MXFP4 weights and x quantized to MXFP8 (laplace_cuda_mxfp4_gemm_dev)."""
+    L = lib()
+    assert x.dtype == torch.float32 and packed.dtype == torch.uint8 and _here(x, packed, y) and M >= 0 and x.numel() >= M * K
+    assert packed.numel() >= L.laplace_cuda_mxfp4_packed_size(1, N, K)
+    if y is None:
+        y = torch.empty((M, N), dtype=torch.float32, device=x.device)
+    assert y.dtype == torch.float32 and y.numel() >= M * N
+    ws = torch.empty(L.laplace_cuda_mxfp4_workspace_size(M, 0, K, N), dtype=torch.uint8, device=x.device)
+    _check(L, L.laplace_cuda_mxfp4_gemm_dev(x.data_ptr(), packed.data_ptr(), y.data_ptr(), M, K, N, ws.data_ptr(), ws.numel(), _stream()))
+    return y
+
+
+def mxfp4_moe_grouped(x: torch.Tensor, packed: torch.Tensor, pair_expert: torch.Tensor, pair_row: torch.Tensor | None,
+                      n_experts_total: int, K: int, N: int, y: torch.Tensor | None = None) -> torch.Tensor:
+    """y[p] = W[pair_expert[p]] . x[pair_row[p]] for (token, expert) pairs in any order, as moe_grouped, with packed MXFP4
+    experts (laplace_cuda_mxfp4_moe_grouped_dev). pair_row None: pair p reads row p. A negative expert leaves its row of y as it was."""
+    L = lib()
+    P = pair_expert.numel()
+    assert K > 0 and pair_expert.dtype == torch.int32 and (pair_row is None or (pair_row.dtype == torch.int32 and pair_row.numel() == P))
+    assert x.dtype == torch.float32 and packed.dtype == torch.uint8 and _here(x, packed, pair_expert, pair_row, y)
+    assert packed.numel() >= L.laplace_cuda_mxfp4_packed_size(n_experts_total, N, K)
+    if y is None:
+        y = torch.empty((P, N), dtype=torch.float32, device=x.device)
+    assert y.dtype == torch.float32 and y.numel() >= P * N
+    ws = torch.empty(L.laplace_cuda_mxfp4_workspace_size(P, n_experts_total, K, N), dtype=torch.uint8, device=x.device)
+    _check(L, L.laplace_cuda_mxfp4_moe_grouped_dev(x.data_ptr(), x.numel() // K, packed.data_ptr(), pair_expert.data_ptr(),
+                                                   pair_row.data_ptr() if pair_row is not None else None, P, n_experts_total, y.data_ptr(), K, N,
+                                                   ws.data_ptr(), ws.numel(), _stream()))
+    return y
+
+
 def sync() -> None:
     """Drains torch's stream and the library's, then surfaces any device-side timeout."""
     torch.cuda.synchronize()

@@ -20,6 +20,7 @@ class GGMLType(enum.IntEnum):
     Q5_K = 13
     Q6_K = 14
     BF16 = 30
+    MXFP4 = 39
 
 
 _GEOM = {
@@ -36,7 +37,7 @@ SUPPORTED = tuple(_GEOM)          # the types with an int8 path (Q8 activations)
 # (elements and bytes per block, Laplace src/tensor.h:41-100)
 ALL_GEOM = dict(_GEOM)
 ALL_GEOM.update({GGMLType.F32: (1, 4), GGMLType.F16: (1, 2), GGMLType.BF16: (1, 2),
-                 GGMLType.Q2_K: (256, 84), GGMLType.Q3_K: (256, 110), GGMLType.Q5_K: (256, 176)})
+                 GGMLType.Q2_K: (256, 84), GGMLType.Q3_K: (256, 110), GGMLType.Q5_K: (256, 176), GGMLType.MXFP4: (32, 17)})
 F32_ACTIVATION_TYPES = (GGMLType.F32, GGMLType.F16, GGMLType.BF16, GGMLType.Q2_K, GGMLType.Q3_K, GGMLType.Q5_K)
 
 
