@@ -14,7 +14,7 @@
 //                                                         (r % 32) * 16 + (r / 32) * 4 + b, the order in which the tensor core takes them
 // A tile is 8 KB in one piece (rows apart would be read 64 bytes at a time), 0.53 bytes per value as in the file.
 // Quantized activations (workspace): image [k tile][row][128 bytes], 16-byte pieces of a row swizzled by row % 8 as the tensor core
-// reads them, and the scales [k tile][128-row group][512 bytes] in the order above.
+// reads them, and the scales [k tile][128-row group][512 bytes] in the order above, the rows of a token tile in groups of their own.
 #include <cuda_bf16.h>
 
 #include "lp_mx.cuh"
@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(512) mxfp4_pack_kernel(const uint8_t* __restri
 // ---- fp32 rows -> MXFP8 image -------------------------------------------------------------------------------------
 // A warp takes 256 values of a row: a 32-value block per 4 lanes. GROUPED: the row of x and the place in the image by pair.
 template <bool GROUPED>
-__global__ void __launch_bounds__(256) mx_act_kernel(const float* __restrict__ x, int K, int kts, int rows, ActDst d, const int* __restrict__ pair_row, const int* __restrict__ dst_row,
+__global__ void __launch_bounds__(256) mx_act_kernel(const float* __restrict__ x, int K, int kts, int rows, ActDst d, const int* __restrict__ pair_row, const int2* __restrict__ place,
                                                      unsigned* __restrict__ counters, int n_counters) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -139,11 +139,14 @@ __global__ void __launch_bounds__(256) mx_act_kernel(const float* __restrict__ x
         for (int i = threadIdx.x; i < n_counters; i += 256) counters[i] = 0;
     const int row = static_cast<int>(id / segs), seg = static_cast<int>(id % segs);
     if (row >= rows) return;
-    int src = row, dst = row;
+    int src = row, dst = row, at;                  // at: row in the groups of scales
     if (GROUPED) {
-        dst = dst_row[row];
+        const int2 p = place[row];
+        dst = p.x; at = p.y;
         if (dst < 0) return;
         if (pair_row) src = pair_row[row];
+    } else {
+        at = row / d.tile_w * (d.tile_groups * 128) + row % d.tile_w;
     }
     const int k = seg * 256 + lane * 8;
     float v[8] = {};
@@ -167,14 +170,13 @@ __global__ void __launch_bounds__(256) mx_act_kernel(const float* __restrict__ x
     const int piece = (lane & 15) >> 1;
     *reinterpret_cast<uint2*>(d.img + (static_cast<size_t>(kt) * d.rows + dst) * 128 + ((piece ^ (dst & 7)) << 4) + (lane & 1) * 8) = q;
     if ((lane & 15) == 0)
-        *reinterpret_cast<uint32_t*>(d.sf + (static_cast<size_t>(kt) * d.groups + (dst >> 7)) * SF_TILE + (dst & 31) * 16 + ((dst >> 5) & 3) * 4) = sc;
+        *reinterpret_cast<uint32_t*>(d.sf + (static_cast<size_t>(kt) * d.groups + (at >> 7)) * SF_TILE + (at & 31) * 16 + ((at >> 5) & 3) * 4) = sc;
 }
 
 // ---- pairs -> places in the image and a table of token tiles --------------------------------------------------------
-// Every block counts all pairs by expert and gives each expert its rows of the image, 32 at a time (a scale byte's place is by row % 32);
-// its warps then walk the pairs of one expert each, in order, so that a pair's place does not depend on timing.
-__global__ void __launch_bounds__(1024) mx_group_kernel(const int* __restrict__ pair_expert, const int* __restrict__ pair_row, int P, int E, int x_rows, int tile_w,
-                                                        int* __restrict__ dst_row, int* __restrict__ out_row, int4* __restrict__ tab, int* __restrict__ n_tiles, int* err) {
+// Every block counts all pairs by expert and gives each expert its rows of the image, 8 at a time, and its token tiles; its warps then walk the pairs of one expert each, in order, so that a pair's place does not depend on timing.
+__global__ void __launch_bounds__(1024) mx_group_kernel(const int* __restrict__ pair_expert, const int* __restrict__ pair_row, int P, int E, int x_rows, int tile_w, int tile_groups,
+                                                        int2* __restrict__ place, int* __restrict__ out_row, int4* __restrict__ tab, int* __restrict__ n_tiles, int* err) {
     extern __shared__ int sm[];
     int* count = sm;
     int* start = sm + E;           // [E + 1]
@@ -193,7 +195,7 @@ __global__ void __launch_bounds__(1024) mx_group_kernel(const int* __restrict__ 
         const int e = expert_of(p);
         if (e >= 0) atomicAdd(count + e, 1);
         else if (blockIdx.x == 0) {
-            dst_row[p] = -1;
+            place[p] = make_int2(-1, -1);
             if (e == -2) atomicCAS(err, DEV_OK, DEV_BAD_INDEX);
         }
     }
@@ -203,7 +205,7 @@ __global__ void __launch_bounds__(1024) mx_group_kernel(const int* __restrict__ 
         int rows = 0, tiles = 0;
         for (int e0 = 0; e0 < E; e0 += 32) {
             const int c = e0 + lane < E ? count[e0 + lane] : 0;
-            int r = (c + 31) & ~31, t = (c + tile_w - 1) / tile_w;
+            int r = (c + 7) & ~7, t = (c + tile_w - 1) / tile_w;
             int ri = r, ti = t;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -220,72 +222,19 @@ __global__ void __launch_bounds__(1024) mx_group_kernel(const int* __restrict__ 
     for (int e = blockIdx.x * 32 + warp; e < E; e += gridDim.x * 32) {
         const int c = count[e], s = start[e];
         if (!c) continue;
-        for (int t = lane; t * tile_w < c; t += 32) tab[tile0[e] + t] = make_int4(e, s + t * tile_w, min(tile_w, c - t * tile_w), 0);
-        int at = s;
+        for (int t = lane; t * tile_w < c; t += 32) tab[tile0[e] + t] = make_int4(e, s + t * tile_w, min(tile_w, c - t * tile_w), (tile0[e] + t) * tile_groups);
+        int at = 0;
         for (int p0 = 0; p0 < P; p0 += 32) {
             const int p = p0 + lane;
             const bool mine = p < P && expert_of(p) == e;
             const unsigned m = __ballot_sync(0xffffffffu, mine);
             if (mine) {
                 const int r = at + __popc(m & ((1u << lane) - 1));
-                dst_row[p] = r;
-                out_row[r] = p;
+                place[p] = make_int2(s + r, (tile0[e] + r / tile_w) * tile_groups * 128 + r % tile_w);
+                out_row[s + r] = p;
             }
             at += __popc(m);
         }
-    }
-}
-
-// ---- the product, simplest form: a thread per weight row, 8 tokens at a time -----------------------------------------
-__device__ __forceinline__ float e2m1_value(uint32_t c) {
-    const float t[8] = {0.f, .5f, 1.f, 1.5f, 2.f, 3.f, 4.f, 6.f};
-    const float m = t[c & 7];
-    return c & 8 ? -m : m;
-}
-template <bool GROUPED>
-__global__ void __launch_bounds__(128) mx_plain_kernel(MxArgs a) {
-    __shared__ float xs[8][128];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int r = threadIdx.x, per_tile = (a.tile_w + 7) / 8;
-    const long long jobs = GROUPED ? static_cast<long long>(*a.n_tiles) * per_tile * a.rts : static_cast<long long>((a.M + 7) / 8) * a.rts;
-    for (long long j = blockIdx.x; j < jobs; j += gridDim.x) {
-        const int rt = static_cast<int>(j % a.rts);
-        int row0, n, e = 0;
-        if (GROUPED) {
-            const int4 t = a.tab[j / a.rts / per_tile];
-            const int off = static_cast<int>(j / a.rts % per_tile) * 8;
-            e = t.x; row0 = t.y + off; n = min(8, t.z - off);
-            if (n <= 0) continue;
-        } else {
-            row0 = static_cast<int>(j / a.rts) * 8;
-            n = min(8, a.M - row0);
-        }
-        float acc[8] = {};
-        for (int kt = 0; kt < a.kts; ++kt) {
-            __syncthreads();
-            for (int i = threadIdx.x; i < n * 128; i += 128) {
-                const int row = row0 + (i >> 7), c = i & 127;
-                const uint8_t q = a.img[(static_cast<size_t>(kt) * a.img_rows + row) * 128 + (((c >> 4) ^ (row & 7)) << 4) + (c & 15)];
-                const uint8_t s = a.sfb[(static_cast<size_t>(kt) * a.groups + (row >> 7)) * SF_TILE + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (c >> 5)];
-                const float f = e4m3_value(q);
-                xs[i >> 7][c] = s == 255 ? __uint_as_float(0x7fc00000u) : f * pow2(static_cast<int>(s) - 127);
-            }
-            __syncthreads();
-            const size_t tile = (static_cast<size_t>(e) * a.rts + rt) * a.kts + kt;
-            for (int b = 0; b < 4; ++b) {
-                const uint4 q = *reinterpret_cast<const uint4*>(a.q + tile * Q_TILE + r * 64 + b * 16);
-                const uint8_t s = a.sfa[tile * SF_TILE + (r & 31) * 16 + (r >> 5) * 4 + b];
-                const float sc = s == 255 ? __uint_as_float(0x7fc00000u) : pow2(static_cast<int>(s) - 127);
-                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-                for (int i = 0; i < 32; ++i) {
-                    const float v = e2m1_value(w[i >> 3] >> (4 * (i & 7))) * sc;
-                    for (int m = 0; m < n; ++m) acc[m] = fmaf(v, xs[m][b * 32 + i], acc[m]);
-                }
-            }
-        }
-        const int col = rt * 128 + r;
-        if (col < a.N)
-            for (int m = 0; m < n; ++m) a.y[static_cast<size_t>(GROUPED ? a.out_row[row0 + m] : row0 + m) * a.N + col] = acc[m];
     }
 }
 
@@ -293,25 +242,31 @@ size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
 // What a call keeps in its workspace, and where.
 struct Plan {
-    int    kts, rts, img_rows, groups, tile_w, max_tiles, n_counters;
-    size_t img, sf, counters, dst_row, out_row, tab, n_tiles, bytes;
+    int    kts, rts, img_rows, groups, nt, tile_w, tile_groups, tiles_m, max_tiles, n_counters;
+    size_t img, sf, counters, part, place, out_row, tab, n_tiles, bytes;
 };
 Plan plan_of(int rows, int experts, int K, int N) {
     Plan p{};
     p.kts = (K + 127) / 128;
     p.rts = (N + 127) / 128;
-    const long long most = experts ? rows + 31ll * (experts < rows ? experts : rows) : rows;
+    const long long most = experts ? rows + 7ll * (experts < rows ? experts : rows) : rows;
     p.img_rows = static_cast<int>((most + 7) & ~7ll);
-    p.groups = (p.img_rows + 127) / 128;
-    p.tile_w = 32;
-    p.max_tiles = experts ? rows / p.tile_w + (experts < rows ? experts : rows) : 0;
+    const int per = experts ? (rows + experts - 1) / experts : rows;
+    p.nt = per <= 32 ? 32 : per <= 64 ? 64 : per <= 128 ? 128 : 256;
+    p.tiles_m = (rows + p.nt - 1) / p.nt;
+    p.tile_w = experts ? p.nt : ((rows + p.tiles_m - 1) / p.tiles_m + 31) & ~31;
+    p.n_counters = ctx().sm_count;
+    p.tile_groups = (p.nt + 127) / 128;
+    p.max_tiles = experts ? rows / p.tile_w + (experts < rows ? experts : rows) : p.tiles_m;
+    p.groups = p.max_tiles * p.tile_groups;
     size_t at = 0;
     auto take = [&](size_t n) { const size_t here = at; at += align256(n); return here; };
     p.img = take(static_cast<size_t>(p.kts) * p.img_rows * 128);
     p.sf = take(static_cast<size_t>(p.kts) * p.groups * SF_TILE);
     p.counters = take(p.n_counters * sizeof(unsigned));
+    p.part = take(mx_gemm_part_bytes(p.nt, experts ? ctx().sm_count : static_cast<int>(static_cast<long long>(p.tiles_m) * p.rts % ctx().sm_count)));
     if (experts) {
-        p.dst_row = take(static_cast<size_t>(rows) * 4);
+        p.place = take(static_cast<size_t>(rows) * sizeof(int2));
         p.out_row = take(static_cast<size_t>(p.img_rows) * 4);
         p.tab = take(static_cast<size_t>(p.max_tiles) * sizeof(int4));
         p.n_tiles = take(4);
@@ -329,27 +284,26 @@ int launch_product(const float* x, int x_rows, const uint8_t* packed, const int*
     a.q = packed;
     a.sfa = packed + static_cast<size_t>(GROUPED ? experts : 1) * p.rts * p.kts * Q_TILE;
     a.img = ws + p.img; a.sfb = ws + p.sf; a.y = y;
-    a.M = rows; a.N = N; a.kts = p.kts; a.rts = p.rts; a.img_rows = p.img_rows; a.groups = p.groups; a.tile_w = p.tile_w;
-    int* dst_row = nullptr;
+    a.M = rows; a.N = N; a.kts = p.kts; a.rts = p.rts; a.img_rows = p.img_rows; a.groups = p.groups; a.tile_w = p.tile_w; a.tiles_m = p.tiles_m; a.tile_groups = p.tile_groups;
+    a.part = reinterpret_cast<float*>(ws + p.part); a.counters = reinterpret_cast<unsigned*>(ws + p.counters); a.err = c.d_err;
+    int2* place = nullptr;
     int rc;
     if (GROUPED) {
-        dst_row = reinterpret_cast<int*>(ws + p.dst_row);
+        place = reinterpret_cast<int2*>(ws + p.place);
         a.out_row = reinterpret_cast<int*>(ws + p.out_row);
         a.tab = reinterpret_cast<int4*>(ws + p.tab);
         a.n_tiles = reinterpret_cast<int*>(ws + p.n_tiles);
-        rc = launch_early(mx_group_kernel, dim3((experts + 31) / 32), 1024, (3 * static_cast<size_t>(experts) + 2) * sizeof(int), st, pair_expert, pair_row, rows, experts, x_rows, p.tile_w,
-                          dst_row, reinterpret_cast<int*>(ws + p.out_row), reinterpret_cast<int4*>(ws + p.tab), reinterpret_cast<int*>(ws + p.n_tiles), c.d_err);
+        rc = launch_early(mx_group_kernel, dim3((experts + 31) / 32), 1024, (3 * static_cast<size_t>(experts) + 2) * sizeof(int), st, pair_expert, pair_row, rows, experts, x_rows, p.tile_w, p.tile_groups,
+                          place, reinterpret_cast<int*>(ws + p.out_row), reinterpret_cast<int4*>(ws + p.tab), reinterpret_cast<int*>(ws + p.n_tiles), c.d_err);
         c.launches++;
         if (rc) return rc;
     }
     const long long warps = static_cast<long long>(rows) * ((p.kts + 1) / 2);
-    rc = launch_early(mx_act_kernel<GROUPED>, dim3(static_cast<unsigned>((warps + 7) / 8)), 256, 0, st, x, K, p.kts, rows, ActDst{ws + p.img, ws + p.sf, p.img_rows, p.groups},
-                      pair_row, static_cast<const int*>(dst_row), reinterpret_cast<unsigned*>(ws + p.counters), p.n_counters);
+    rc = launch_early(mx_act_kernel<GROUPED>, dim3(static_cast<unsigned>((warps + 7) / 8)), 256, 0, st, x, K, p.kts, rows, ActDst{ws + p.img, ws + p.sf, p.img_rows, p.groups, p.tile_w, p.tile_groups},
+                      pair_row, static_cast<const int2*>(place), reinterpret_cast<unsigned*>(ws + p.counters), p.n_counters);
     c.launches++;
     if (rc) return rc;
-    rc = launch_early(mx_plain_kernel<GROUPED>, dim3(c.sm_count * 8), 128, 0, st, a);
-    c.launches++;
-    return rc;
+    return launch_mx_gemm(a, p.nt, static_cast<long long>(GROUPED ? experts : 1) * p.rts * p.kts, GROUPED, st);
 }
 
 int bad_shape(const char* what, int K, int N, long long experts) {
@@ -362,8 +316,6 @@ bool misaligned(const void* p, unsigned n) { return reinterpret_cast<uintptr_t>(
 constexpr int MAX_EXPERTS = 4000;      // three counters each in 48 KB of shared memory
 
 }  // namespace
-
-int launch_mxfp4_dequantize(const uint8_t* w, float* dst, long long n, float scale, cudaStream_t st);
 
 }  // namespace lp
 
@@ -416,7 +368,7 @@ int laplace_cuda_mxfp4_pack_dev(const uint8_t* w, uint8_t* packed, int n_experts
 }
 
 size_t laplace_cuda_mxfp4_workspace_size(int rows, int n_experts, int K, int N) {
-    if (rows <= 0 || n_experts < 0 || K <= 0 || N <= 0 || K % 32) return 0;
+    if (!ctx().ready || rows <= 0 || n_experts < 0 || K <= 0 || N <= 0 || K % 32) return 0;
     return plan_of(rows, n_experts, K, N).bytes;
 }
 
