@@ -25,35 +25,6 @@ namespace {
 using namespace mx;
 
 // ---- values -> GGUF blocks ---------------------------------------------------------------------------------------
-template <class T> __device__ __forceinline__ void load8(const T* p, float (&v)[8]);
-template <> __device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-template <> __device__ __forceinline__ void load8<__half>(const __half* p, float (&v)[8]) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        v[2 * i] = f.x; v[2 * i + 1] = f.y;
-    }
-}
-template <> __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&v)[8]) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-}
-__device__ __forceinline__ float amax8(const float (&v)[8]) {
-    float a = fabsf(v[0]);
-#pragma unroll
-    for (int i = 1; i < 8; ++i) a = max_nan(a, fabsf(v[i]));
-    return a;
-}
-// 2^e for e in [-127, 127]
-__device__ __forceinline__ float pow2(int e) { return e == -127 ? __uint_as_float(0x00400000u) : __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
-
 // A block per 4 lanes, 8 values each; 64 blocks a CTA, gathered in shared memory and written in order.
 constexpr int QB = 64;
 template <class T>
@@ -126,6 +97,9 @@ __global__ void __launch_bounds__(512) mxfp4_pack_kernel(const uint8_t* __restri
     sf[tile * SF_TILE + (r & 31) * 16 + (r >> 5) * 4 + b] = scale;
 }
 
+// What follows in the stream may read the tiles before it has waited for the kernel before it: that is this one, which begins when the tiles are written.
+__global__ void mxfp4_packed_kernel() {}
+
 // ---- fp32 rows -> MXFP8 image -------------------------------------------------------------------------------------
 // A warp takes 256 values of a row: a 32-value block per 4 lanes. GROUPED: the row of x and the place in the image by pair.
 template <bool GROUPED>
@@ -151,20 +125,8 @@ __global__ void __launch_bounds__(256) mx_act_kernel(const float* __restrict__ x
     const int k = seg * 256 + lane * 8;
     float v[8] = {};
     if (k < K) load8(x + static_cast<size_t>(src) * K + k, v);         // K is a multiple of 32: all eight or none
-    float a = amax8(v);
-    a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 1));
-    a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 2));
-    const bool bad = !(a < __uint_as_float(0x7f800000u));
-    const uint32_t bits = __float_as_uint(a);
-    int s = static_cast<int>(bits >> 23) - 135 + ((bits & 0x7fffffu) > 0x600000u);      // a = m 2^e, 1 <= m < 2: e - 8 up to m = 1.75, else e - 7
-    if (s < -127) s = -127;
-    const float inv = pow2(-s);
-    uint2 q;
-    q.x = bad ? 0x7f7f7f7fu : e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-    q.y = bad ? 0x7f7f7f7fu : e4m3x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
-    uint32_t sc = (bad ? 255u : static_cast<uint32_t>(s + 127)) << (8 * ((lane >> 2) & 3));
-    sc |= __shfl_xor_sync(0xffffffffu, sc, 4);
-    sc |= __shfl_xor_sync(0xffffffffu, sc, 8);
+    uint32_t sc;
+    const uint2 q = mxfp8_block8(v, lane, sc);
     const int kt = seg * 2 + (lane >> 4);
     if (kt >= kts) return;
     const int piece = (lane & 15) >> 1;
@@ -278,6 +240,7 @@ Plan plan_of(int rows, int experts, int K, int N) {
 template <bool GROUPED>
 int launch_product(const float* x, int x_rows, const uint8_t* packed, const int* pair_expert, const int* pair_row, int rows, int experts, float* y, int K, int N,
                    uint8_t* ws, cudaStream_t st) {
+    if (mx_small_takes(rows, GROUPED)) return launch_mx_small(x, x_rows, packed, pair_expert, pair_row, rows, experts, y, K, N, st);
     const Plan p = plan_of(rows, GROUPED ? experts : 0, K, N);
     Context& c = ctx();
     MxArgs a{};
@@ -364,6 +327,8 @@ int laplace_cuda_mxfp4_pack_dev(const uint8_t* w, uint8_t* packed, int n_experts
                                                                                 packed + n_tiles * Q_TILE + t0 * SF_TILE, N, K, rts, kts);
         ctx().launches++;
     }
+    mxfp4_packed_kernel<<<1, 32, 0, MX_STREAM(stream)>>>();
+    ctx().launches++;
     return cuda_check(cudaGetLastError(), "mxfp4_pack launch");
 }
 

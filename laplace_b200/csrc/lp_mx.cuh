@@ -1,6 +1,8 @@
 // lp_mx.cuh - what the MXFP4 kernels share: sizes of the packed layout (lp_mx.cu), conversions, arguments of a product.
 #pragma once
 
+#include <cuda_bf16.h>
+
 #include "lp_common.cuh"
 
 namespace lp {
@@ -45,6 +47,54 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(hi) : "f"(c), "f"(d));
     return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
 }
+template <class T> __device__ __forceinline__ void load8(const T* p, float (&v)[8]);
+template <> __device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+template <> __device__ __forceinline__ void load8<__half>(const __half* p, float (&v)[8]) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        v[2 * i] = f.x; v[2 * i + 1] = f.y;
+    }
+}
+template <> __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&v)[8]) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+}
+__device__ __forceinline__ float amax8(const float (&v)[8]) {
+    float a = fabsf(v[0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) a = max_nan(a, fabsf(v[i]));
+    return a;
+}
+// 2^e for e in [-127, 127]
+__device__ __forceinline__ float pow2(int e) { return e == -127 ? __uint_as_float(0x00400000u) : __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+
+// Eight values of a 32-value block that four neighbouring lanes hold -> their e4m3 bytes; sc: the scale bytes of the lane's 16-lane half
+// (128 values), lowest block first. A block with an infinity or a NaN is NaN, scale and values.
+__device__ __forceinline__ uint2 mxfp8_block8(const float (&v)[8], int lane, uint32_t& sc) {
+    float a = amax8(v);
+    a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 1));
+    a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 2));
+    const bool bad = !(a < __uint_as_float(0x7f800000u));
+    const uint32_t bits = __float_as_uint(a);
+    int s = static_cast<int>(bits >> 23) - 135 + ((bits & 0x7fffffu) > 0x600000u);      // a = m 2^e, 1 <= m < 2: e - 8 up to m = 1.75, else e - 7
+    if (s < -127) s = -127;
+    const float inv = pow2(-s);
+    uint2 q;
+    q.x = bad ? 0x7f7f7f7fu : e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+    q.y = bad ? 0x7f7f7f7fu : e4m3x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+    sc = (bad ? 255u : static_cast<uint32_t>(s + 127)) << (8 * ((lane >> 2) & 3));
+    sc |= __shfl_xor_sync(0xffffffffu, sc, 4);
+    sc |= __shfl_xor_sync(0xffffffffu, sc, 8);
+    return q;
+}
 
 #endif
 
@@ -53,6 +103,8 @@ constexpr int MIN_STEPS = 2;          // least k steps of 128 that a CTA takes o
 }  // namespace mx
 
 size_t mx_gemm_part_bytes(int nt, int cut_tiles);
+bool   mx_small_takes(int rows, bool grouped);
+int    launch_mx_small(const float* x, int x_rows, const uint8_t* packed, const int* pair_expert, const int* pair_row, int rows, int experts, float* y, int K, int N, cudaStream_t st);
 int    launch_mx_gemm(const mx::MxArgs& a, int nt, long long tiles, bool grouped, cudaStream_t st);
 
 }  // namespace lp

@@ -11,6 +11,7 @@
 // Roles by warp: 0 copies, 1 MMA issue (owns the TMEM), 4-7 drain (lane = weight row). All waits are bounded; a wait that gives up
 // raises the status word and the roles leave their loops.
 #include "lp_mx.cuh"
+#include "lp_mx_mma.cuh"
 #include "lp_tc.cuh"
 
 namespace lp {
@@ -102,22 +103,6 @@ struct Walk {
     }
 };
 
-// kind::mxf8f6f4: D fp32, A e2m1, B e4m3, both K-major, scales ue8m0; 128 rows of A, n of B; the byte of the scale words that this step takes
-__device__ __forceinline__ uint32_t idesc_mx(int n, int byte) {
-    return (static_cast<uint32_t>(byte) << 4) | (5u << 7) | (0u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) | (8u << 24) | (static_cast<uint32_t>(byte) << 29);
-}
-__device__ __forceinline__ void mma_mx(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t acc) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-        :: "r"(d), "l"(ad), "l"(bd), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc) : "memory");
-}
-// 32 rows of 16 bytes -> 4 TMEM columns of every quadrant
-__device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t smem) {
-    const uint64_t d = static_cast<uint64_t>((smem >> 4) & 0x3fffu) | (static_cast<uint64_t>(128 >> 4) << 16) | (static_cast<uint64_t>(128 >> 4) << 32) | (static_cast<uint64_t>(1) << 46);
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" :: "r"(taddr), "l"(d) : "memory");
-}
-
 template <int NT, bool GROUPED>
 __global__ void __launch_bounds__(THREADS, 1) mx_gemm_kernel(const __grid_constant__ CUtensorMap map, const MxArgs a) {
     using L = Lay<NT>;
@@ -125,7 +110,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx_gemm_kernel(const __grid_consta
     const uint32_t sb = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem = smem_raw + (sb - smem_u32(smem_raw));
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::ABORT);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::STAGES; ++i) { mbar_init(sb + L::FULL + 8 * i, 1); mbar_init(sb + L::EMPTY + 8 * i, 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(sb + L::TFULL + 8 * i, 1); mbar_init(sb + L::TEMPTY + 8 * i, 128); }
@@ -146,7 +131,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx_gemm_kernel(const __grid_consta
     if (GROUPED || warp != 0) asm volatile("griddepcontrol.wait;" ::: "memory");
     const Work w = work_of(GROUPED ? static_cast<long long>(*a.n_tiles) * a.rts : static_cast<long long>(a.tiles_m) * a.rts, a.kts, gridDim.x);
 
-    if (warp == 0 && lane == 0) {
+    if (warp == 0 && elect_one()) {
         auto tile_of = [&](const Seg& s, int kt) { return (static_cast<size_t>(s.expert) * a.rts + s.rt) * a.kts + kt; };
         auto weights = [&](int st, const Seg& s, int kt) {
             const int n8 = (s.n + 7) & ~7, groups = (s.n + 127) >> 7;
@@ -183,7 +168,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx_gemm_kernel(const __grid_consta
             }
         if (!ok)                                        // what is in flight lands before the CTA goes
             for (int i = 0; i < 1000; ++i) __nanosleep(1000);
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1 && elect_one()) {
         Walk<GROUPED> walk(a, w);
         Seg s;
         int it = 0;
@@ -295,8 +280,7 @@ size_t mx_gemm_part_bytes(int nt, int cut_tiles) { return static_cast<size_t>(ct
 
 int launch_mx_gemm(const MxArgs& a, int nt, long long tiles, bool grouped, cudaStream_t st) {
     CUtensorMap map;
-    // the tiles' rows one after the other: 128 values, 64 bytes each
-    if (!make_map_2d(&map, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, a.q, 128, static_cast<uint64_t>(tiles) * 128, 64, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B, "MXFP4 weights")) return LAPLACE_ERR_CUDA;
+    if (!mx_weights_map(&map, a.q, static_cast<size_t>(tiles))) return LAPLACE_ERR_CUDA;
     if (grouped) switch (nt) {
         case 32: return launch_nt<32, true>(map, a, st);
         case 64: return launch_nt<64, true>(map, a, st);
