@@ -136,68 +136,99 @@ __global__ void __launch_bounds__(256) mx_act_kernel(const float* __restrict__ x
 }
 
 // ---- pairs -> places in the image and a table of token tiles --------------------------------------------------------
-// Every block counts all pairs by expert and gives each expert its rows of the image, 8 at a time, and its token tiles; its warps then walk the pairs of one expert each, in order, so that a pair's place does not depend on timing.
+// One block. Every warp has a run of the pairs and counts them by expert; the counts, summed over the warps before it, are where its pairs
+// of an expert begin, so that a pair's place is by its number and not by timing. An expert gets whole groups of 8 rows of the image
+// and token tiles of its own. (A warp per expert walking all pairs: 158 us for 16,384 pairs and 128 experts, 32 of them to a block.)
+__device__ __forceinline__ int pair_expert_of(const int* pair_expert, const int* pair_row, int p, int P, int E, int x_rows) {
+    if (p >= P) return -1;
+    const int e = __ldg(pair_expert + p);
+    if (e < 0) return -1;
+    return e >= E || (pair_row && static_cast<unsigned>(__ldg(pair_row + p)) >= static_cast<unsigned>(x_rows)) ? -2 : e;
+}
 __global__ void __launch_bounds__(1024) mx_group_kernel(const int* __restrict__ pair_expert, const int* __restrict__ pair_row, int P, int E, int x_rows, int tile_w, int tile_groups,
                                                         int2* __restrict__ place, int* __restrict__ out_row, int4* __restrict__ tab, int* __restrict__ n_tiles, int* err) {
     extern __shared__ int sm[];
-    int* count = sm;
-    int* start = sm + E;           // [E + 1]
-    int* tile0 = sm + 2 * E + 1;   // [E + 1]
+    const int W = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int* start = sm;                       // first row of an expert in the image
+    int* tile0 = sm + E;                   // its first token tile
+    int* count = sm + 2 * E;               // [W][E]: the warp's pairs of an expert, then where they begin among the expert's
+    for (int i = threadIdx.x; i < W * E; i += blockDim.x) count[i] = 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    for (int i = threadIdx.x; i < E; i += blockDim.x) count[i] = 0;
     __syncthreads();
-    auto expert_of = [&](int p) {
-        const int e = __ldg(pair_expert + p);
-        if (e < 0) return -1;
-        if (e >= E || (pair_row && static_cast<unsigned>(__ldg(pair_row + p)) >= static_cast<unsigned>(x_rows))) return -2;
-        return e;
-    };
-    for (int p = threadIdx.x; p < P; p += blockDim.x) {
-        const int e = expert_of(p);
-        if (e >= 0) atomicAdd(count + e, 1);
-        else if (blockIdx.x == 0) {
-            place[p] = make_int2(-1, -1);
-            if (e == -2) atomicCAS(err, DEV_OK, DEV_BAD_INDEX);
+    const int run = ((P + W - 1) / W + 31) & ~31, p0 = warp * run, p1 = min(p0 + run, P);
+    int* mine = count + warp * E;
+    const unsigned before = (1u << lane) - 1;
+    constexpr int U = 8;                   // loads of so many steps at once
+    for (int q = p0; q < p1; q += 32 * U) {
+        int e[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) e[i] = pair_expert_of(pair_expert, pair_row, q + 32 * i + lane, p1, E, x_rows);
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const unsigned same = __match_any_sync(0xffffffffu, e[i]);
+            if (e[i] >= 0 && !(same & before)) mine[e[i]] += __popc(same);
+            __syncwarp();
         }
     }
     __syncthreads();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int e = threadIdx.x; e < E; e += blockDim.x) {
+        int sum = 0;
+        for (int v = 0; v < W; ++v) { const int c = count[v * E + e]; count[v * E + e] = sum; sum += c; }
+        start[e] = sum;
+    }
+    __syncthreads();
     if (warp == 0) {
         int rows = 0, tiles = 0;
         for (int e0 = 0; e0 < E; e0 += 32) {
-            const int c = e0 + lane < E ? count[e0 + lane] : 0;
-            int r = (c + 7) & ~7, t = (c + tile_w - 1) / tile_w;
+            const int c = e0 + lane < E ? start[e0 + lane] : 0;
+            const int r = (c + 7) & ~7, t = (c + tile_w - 1) / tile_w;
             int ri = r, ti = t;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int a = __shfl_up_sync(0xffffffffu, ri, o), b = __shfl_up_sync(0xffffffffu, ti, o);
                 if (lane >= o) { ri += a; ti += b; }
             }
-            if (e0 + lane < E) { start[e0 + lane] = rows + ri - r; tile0[e0 + lane] = tiles + ti - t; }
+            if (e0 + lane < E) {
+                const int s = rows + ri - r, t0 = tiles + ti - t;
+                start[e0 + lane] = s;
+                tile0[e0 + lane] = t0;
+                for (int i = 0; i < t; ++i) tab[t0 + i] = make_int4(e0 + lane, s + i * tile_w, min(tile_w, c - i * tile_w), (t0 + i) * tile_groups);
+            }
             rows += __shfl_sync(0xffffffffu, ri, 31);
             tiles += __shfl_sync(0xffffffffu, ti, 31);
         }
-        if (lane == 0 && blockIdx.x == 0) *n_tiles = tiles;
+        if (lane == 0) *n_tiles = tiles;
     }
     __syncthreads();
-    for (int e = blockIdx.x * 32 + warp; e < E; e += gridDim.x * 32) {
-        const int c = count[e], s = start[e];
-        if (!c) continue;
-        for (int t = lane; t * tile_w < c; t += 32) tab[tile0[e] + t] = make_int4(e, s + t * tile_w, min(tile_w, c - t * tile_w), (tile0[e] + t) * tile_groups);
-        int at = 0;
-        for (int p0 = 0; p0 < P; p0 += 32) {
-            const int p = p0 + lane;
-            const bool mine = p < P && expert_of(p) == e;
-            const unsigned m = __ballot_sync(0xffffffffu, mine);
-            if (mine) {
-                const int r = at + __popc(m & ((1u << lane) - 1));
-                place[p] = make_int2(s + r, (tile0[e] + r / tile_w) * tile_groups * 128 + r % tile_w);
-                out_row[s + r] = p;
+    for (int q = p0; q < p1; q += 32 * U) {
+        int e[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) e[i] = pair_expert_of(pair_expert, pair_row, q + 32 * i + lane, p1, E, x_rows);
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int p = q + 32 * i + lane;
+            const unsigned same = __match_any_sync(0xffffffffu, e[i]);
+            const int base = e[i] >= 0 ? mine[e[i]] : 0;
+            __syncwarp();
+            if (e[i] >= 0) {
+                const int r = base + __popc(same & before);
+                place[p] = make_int2(start[e[i]] + r, (tile0[e[i]] + r / tile_w) * tile_groups * 128 + r % tile_w);
+                out_row[start[e[i]] + r] = p;
+                if (!(same & before)) mine[e[i]] = base + __popc(same);
+            } else if (p < p1) {
+                place[p] = make_int2(-1, -1);
+                if (e[i] == -2) atomicCAS(err, DEV_OK, DEV_BAD_INDEX);
             }
-            at += __popc(m);
+            __syncwarp();
         }
     }
+}
+constexpr int MAX_EXPERTS = 4000;
+// warps of the grouping block: 32, or as many as leave their counters room in shared memory (200 KB in all)
+int group_warps(int experts) {
+    const int w = (200 * 1024 / 4 - 2 * experts) / experts;
+    return w < 32 ? w : 32;
 }
 
 size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
@@ -256,8 +287,14 @@ int launch_product(const float* x, int x_rows, const uint8_t* packed, const int*
         a.out_row = reinterpret_cast<int*>(ws + p.out_row);
         a.tab = reinterpret_cast<int4*>(ws + p.tab);
         a.n_tiles = reinterpret_cast<int*>(ws + p.n_tiles);
-        rc = launch_early(mx_group_kernel, dim3((experts + 31) / 32), 1024, (3 * static_cast<size_t>(experts) + 2) * sizeof(int), st, pair_expert, pair_row, rows, experts, x_rows, p.tile_w, p.tile_groups,
-                          place, reinterpret_cast<int*>(ws + p.out_row), reinterpret_cast<int4*>(ws + p.tab), reinterpret_cast<int*>(ws + p.n_tiles), c.d_err);
+        const int warps = group_warps(experts);
+        static bool configured = false;
+        if (!configured) {
+            if ((rc = cuda_check(cudaFuncSetAttribute(mx_group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024), "mx_group shared memory"))) return rc;
+            configured = true;
+        }
+        rc = launch_early(mx_group_kernel, dim3(1), warps * 32, (warps + 2) * static_cast<size_t>(experts) * sizeof(int), st, pair_expert, pair_row, rows, experts, x_rows, p.tile_w,
+                          p.tile_groups, place, reinterpret_cast<int*>(ws + p.out_row), reinterpret_cast<int4*>(ws + p.tab), reinterpret_cast<int*>(ws + p.n_tiles), c.d_err);
         c.launches++;
         if (rc) return rc;
     }
@@ -276,7 +313,6 @@ int bad_shape(const char* what, int K, int N, long long experts) {
     return LAPLACE_OK;
 }
 bool misaligned(const void* p, unsigned n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }
-constexpr int MAX_EXPERTS = 4000;      // three counters each in 48 KB of shared memory
 
 }  // namespace
 

@@ -8,7 +8,7 @@
 // of a tile leaves its sums in the workspace; the last of a tile's CTAs to arrive (a counter) adds them up in the order of k, so that the
 // result does not depend on who was last. Few rows (decode) are all cut: every SM streams the same share of the weights.
 //
-// Roles by warp: 0 copies, 1 MMA issue (owns the TMEM), 4-7 drain (lane = weight row). All waits are bounded; a wait that gives up
+// Roles by warp: 0 copies, 1 MMA issue (owns the TMEM), 4-11 drain (lane = weight row). All waits are bounded; a wait that gives up
 // raises the status word and the roles leave their loops.
 #include "lp_mx.cuh"
 #include "lp_mx_mma.cuh"
@@ -20,7 +20,8 @@ namespace {
 using namespace mx;
 using namespace tc;
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 384;
+constexpr int DRAIN = 256;                     // threads of the drain: two warps per quadrant of TMEM lanes
 constexpr int A_STAGE = 128 * 128;             // 128 rows x 128 values, a byte each after the copy
 constexpr uint32_t SF_COL = 480;               // TMEM columns of the scales: two sets of 16 (4 of the weights, up to 8 of the activations)
 
@@ -113,7 +114,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx_gemm_kernel(const __grid_consta
     const int warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::STAGES; ++i) { mbar_init(sb + L::FULL + 8 * i, 1); mbar_init(sb + L::EMPTY + 8 * i, 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(sb + L::TFULL + 8 * i, 1); mbar_init(sb + L::TEMPTY + 8 * i, 128); }
+        for (int i = 0; i < 2; ++i) { mbar_init(sb + L::TFULL + 8 * i, 1); mbar_init(sb + L::TEMPTY + 8 * i, DRAIN / 32); }
         *abort_flag = 0;
         fence_barrier_init();
         asm volatile("prefetch.tensormap [%0];" :: "l"(&map) : "memory");
@@ -196,7 +197,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx_gemm_kernel(const __grid_consta
     } else if (warp >= 4) {
         Walk<GROUPED> walk(a, w);
         Seg s;
-        const int r = threadIdx.x - 128;                // weight row of the tile
+        const int lane = threadIdx.x & 31, id = threadIdx.x - 128, half = id >> 7, r = id & 127;      // r: weight row of the tile
         const uint32_t quadrant = static_cast<uint32_t>(warp & 3) * 32u << 16;
         volatile int* last = reinterpret_cast<volatile int*>(smem + L::LAST);
         for (int seg = 0; walk(s); ++seg) {
@@ -205,50 +206,88 @@ __global__ void __launch_bounds__(THREADS, 1) mx_gemm_kernel(const __grid_consta
             __syncwarp();
             fence_after();
             const int col = s.rt * 128 + r;
-            auto out = [&](int m, float v) {
-                if (col < a.N) a.y[static_cast<size_t>(GROUPED ? __ldg(a.out_row + s.row0 + m) : s.row0 + m) * a.N + col] = v;
-            };
             float* part = a.part + static_cast<size_t>(blockIdx.x + max(s.cut, 0)) * (NT * 128) + r;
-            for (int c0 = 0; c0 < s.n; c0 += 32) {
+            for (int c0 = 32 * half; c0 < s.n; c0 += 64) {
                 float v[32];
+                const int here = min(32, s.n - c0);
+                int to = 0;                             // lane: the row of y that column c0 + lane goes to
+                if (GROUPED && s.cut < 0 && lane < here) to = __ldg(a.out_row + s.row0 + c0 + lane);
                 __syncwarp();
                 ld32(tmem + quadrant + acc * NT + c0, v);
                 wait_ld();
+                if (s.cut >= 0) {
+                    float* q = part + c0 * 128;
+                    if (here == 32) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    if (c0 + i >= s.n) break;
-                    if (s.cut < 0) out(c0 + i, v[i]);
-                    else __stcg(part + (c0 + i) * 128, v[i]);
+                        for (int i = 0; i < 32; ++i) __stcg(q + i * 128, v[i]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (i < here) __stcg(q + i * 128, v[i]);
+                    }
+                } else if (GROUPED) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int m = __shfl_sync(0xffffffffu, to, i);
+                        if (i < here && col < a.N) a.y[static_cast<size_t>(m) * a.N + col] = v[i];
+                    }
+                } else {
+                    float* q = a.y + static_cast<size_t>(s.row0 + c0) * a.N + col;
+                    if (here == 32 && col < a.N) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) q[static_cast<size_t>(i) * a.N] = v[i];
+                    } else if (col < a.N) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (i < here) q[static_cast<size_t>(i) * a.N] = v[i];
+                    }
                 }
             }
             fence_before();
-            mbar_arrive(sb + L::TEMPTY + 8 * acc);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sb + L::TEMPTY + 8 * acc);
             if (s.cut < 0) continue;
             const long long u = static_cast<long long>(s.cut) * a.kts;
             const int first = cut_owner(w, u), pieces = cut_owner(w, u + a.kts - 1) - first + 1;
             __threadfence();
-            named_bar_sync(1, 128);
-            if (r == 0) *last = atomicAdd(a.counters + s.cut, 1u) == static_cast<unsigned>(pieces - 1);
-            named_bar_sync(1, 128);
+            named_bar_sync(1, DRAIN);
+            if (id == 0) *last = atomicAdd(a.counters + s.cut, 1u) == static_cast<unsigned>(pieces - 1);
+            named_bar_sync(1, DRAIN);
             if (!*last) continue;
             __threadfence();
-            const float* p0 = a.part + static_cast<size_t>(first + s.cut) * (NT * 128) + r;
-            for (int c0 = 0; c0 < s.n; c0 += 4) {
-                float sum[4] = {};
-                for (int p = 0; p < pieces; p += 8) {
-                    float v[8][4];
+            // four rows of a column a thread, eight columns at a time; parts in the order of k
+            const int r4 = (id & 31) * 4, col4 = s.rt * 128 + r4;
+            const float* p0 = a.part + static_cast<size_t>(first + s.cut) * (NT * 128) + r4;
+            const bool vec = (a.N & 3) == 0 && (reinterpret_cast<uintptr_t>(a.y) & 15) == 0;
+            for (int c0 = id >> 5; c0 < s.n; c0 += 32) {
+                float4 sum[4] = {};
+                for (int p = 0; p < pieces; p += 4) {
+                    float4 v[4][4];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
+                    for (int i = 0; i < 4; ++i)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) v[i][j] = p + i < pieces && c0 + j < s.n ? __ldcg(p0 + static_cast<size_t>(p + i) * (NT * 128) + (c0 + j) * 128) : 0.f;
+                        for (int j = 0; j < 4; ++j)
+                            v[i][j] = p + i < pieces && c0 + 8 * j < s.n ? __ldcg(reinterpret_cast<const float4*>(p0 + static_cast<size_t>(p + i) * (NT * 128) + (c0 + 8 * j) * 128))
+                                                                          : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
+                    for (int i = 0; i < 4; ++i)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) sum[j] += v[i][j];
+                        for (int j = 0; j < 4; ++j) { sum[j].x += v[i][j].x; sum[j].y += v[i][j].y; sum[j].z += v[i][j].z; sum[j].w += v[i][j].w; }
                 }
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (c0 + j < s.n) out(c0 + j, sum[j]);
+                for (int j = 0; j < 4; ++j) {
+                    const int m = c0 + 8 * j;
+                    if (m >= s.n) break;
+                    float* q = a.y + static_cast<size_t>(GROUPED ? __ldg(a.out_row + s.row0 + m) : s.row0 + m) * a.N + col4;
+                    if (vec) {
+                        if (col4 < a.N) *reinterpret_cast<float4*>(q) = sum[j];
+                    } else {
+                        const float e[4] = {sum[j].x, sum[j].y, sum[j].z, sum[j].w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (col4 + i < a.N) q[i] = e[i];
+                    }
+                }
             }
         }
     }
