@@ -24,6 +24,12 @@ struct Entries {
     decltype(&laplace_cuda_lm_head_dev) lm_head;
     decltype(&laplace_cuda_moe_route_dev) moe_route;
     decltype(&laplace_cuda_moe_ffn_dev) moe_ffn;
+    decltype(&laplace_cuda_dequantize_dev) dequantize;
+    decltype(&laplace_cuda_mxfp4_quantize_dev) mxfp4_quantize;
+    decltype(&laplace_cuda_mxfp4_packed_size) mxfp4_packed_size;
+    decltype(&laplace_cuda_mxfp4_workspace_size) mxfp4_workspace_size;
+    decltype(&laplace_cuda_mxfp4_gemm_dev) mxfp4_gemm;
+    decltype(&laplace_cuda_mxfp4_moe_grouped_dev) mxfp4_moe_grouped;
 } g;
 int g_device = -1;
 
@@ -40,6 +46,7 @@ void block_of(long type, long& elems, long& bytes) {
         case 12: elems = 256; bytes = 144; break;        // Q4_K
         case 13: elems = 256; bytes = 176; break;        // Q5_K
         case 14: elems = 256; bytes = 210; break;        // Q6_K
+        case 39: elems = 32; bytes = 17; break;          // MXFP4
         default: elems = 0; bytes = 0;
     }
 }
@@ -237,23 +244,111 @@ PyObject* py_moe_ffn(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
-// bind(device, addresses of the six entry points in the order of Entries)
+// dequantize(w, type, n)
+PyObject* py_dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const at::Tensor* w;
+        long type, count;
+        if (n != 3 || !ready() || !tensor(a[0], at::kByte, w) || !number(a[1], type) || !number(a[2], count) || !whole_rows(*w, type, count, 1)) Py_RETURN_NONE;
+        const at::Tensor out = fresh({count}, at::kFloat);
+        const auto* pw = ptr<const uint8_t>(*w);
+        auto* po = ptr<float>(out);
+        void* st = stream();
+        if (unlocked([&] { return g.dequantize(pw, type, po, count, st); }))
+            Py_RETURN_NONE;
+        return THPVariable_Wrap(out);
+    });
+}
+
+// mxfp4_quantize(x)
+PyObject* py_mxfp4_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const at::Tensor* x;
+        if (n != 1 || !ready() || !(tensor(a[0], at::kFloat, x) || tensor(a[0], at::kHalf, x) || tensor(a[0], at::kBFloat16, x)) || x->dim() < 1 || x->size(-1) % 32) Py_RETURN_NONE;
+        const uint32_t type = x->scalar_type() == at::kFloat ? 0 : x->scalar_type() == at::kHalf ? 1 : 30;
+        const long count = x->numel();
+        const at::Tensor out = fresh({count / 32 * 17}, at::kByte);
+        const void* px = x->data_ptr();
+        auto* po = ptr<uint8_t>(out);
+        void* st = stream();
+        if (unlocked([&] { return g.mxfp4_quantize(px, type, po, count, st); }))
+            Py_RETURN_NONE;
+        return THPVariable_Wrap(out);
+    });
+}
+
+// mxfp4_gemm(x, packed, M, K, N, y or None)
+PyObject* py_mxfp4_gemm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const at::Tensor *x, *w, *y = nullptr;
+        long M, K, N;
+        if (n != 6 || !ready() || !tensor(a[0], at::kFloat, x) || !tensor(a[1], at::kByte, w) || !number(a[2], M) || !number(a[3], K) || !number(a[4], N) ||
+            (a[5] != Py_None && !tensor(a[5], at::kFloat, y)) || K <= 0 || N <= 0 || K % 32 || x->numel() < M * K || (y && y->numel() < M * N) ||
+            static_cast<size_t>(w->numel()) < g.mxfp4_packed_size(1, N, K))
+            Py_RETURN_NONE;
+        const at::Tensor out = y ? *y : fresh({M, N}, at::kFloat);
+        const long bytes = static_cast<long>(g.mxfp4_workspace_size(M, 0, K, N));
+        const at::Tensor ws = fresh({bytes}, at::kByte);
+        const auto* px = ptr<const float>(*x);
+        const auto* pw = ptr<const uint8_t>(*w);
+        auto* po = ptr<float>(out);
+        void *pws = ws.data_ptr(), *st = stream();
+        if (unlocked([&] { return g.mxfp4_gemm(px, pw, po, M, K, N, pws, bytes, st); }))
+            Py_RETURN_NONE;
+        if (y) { Py_INCREF(a[5]); return a[5]; }
+        return THPVariable_Wrap(out);
+    });
+}
+
+// mxfp4_moe_grouped(x, packed, pair_expert, pair_row or None, experts, K, N, y or None)
+PyObject* py_mxfp4_moe_grouped(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const at::Tensor *x, *w, *idx, *row = nullptr, *y = nullptr;
+        long E, K, N;
+        if (n != 8 || !ready() || !tensor(a[0], at::kFloat, x) || !tensor(a[1], at::kByte, w) || !tensor(a[2], at::kInt, idx) || (a[3] != Py_None && !tensor(a[3], at::kInt, row)) ||
+            !number(a[4], E) || !number(a[5], K) || !number(a[6], N) || (a[7] != Py_None && !tensor(a[7], at::kFloat, y)) || E <= 0 || K <= 0 || N <= 0 || K % 32 ||
+            (row && row->numel() != idx->numel()) || static_cast<size_t>(w->numel()) < g.mxfp4_packed_size(E, N, K))
+            Py_RETURN_NONE;
+        const long P = idx->numel(), rows = x->numel() / K;
+        if (P >= 1L << 31 || rows >= 1L << 31 || (y && y->numel() < P * N)) Py_RETURN_NONE;
+        const at::Tensor out = y ? *y : fresh({P, N}, at::kFloat);
+        const long bytes = static_cast<long>(g.mxfp4_workspace_size(P, E, K, N));
+        const at::Tensor ws = fresh({bytes}, at::kByte);
+        const auto* px = ptr<const float>(*x);
+        const auto* pw = ptr<const uint8_t>(*w);
+        const auto *pi = ptr<const int>(*idx), *pr = row ? ptr<const int>(*row) : nullptr;
+        auto* po = ptr<float>(out);
+        void *pws = ws.data_ptr(), *st = stream();
+        if (unlocked([&] { return g.mxfp4_moe_grouped(px, rows, pw, pi, pr, P, E, po, K, N, pws, bytes, st); }))
+            Py_RETURN_NONE;
+        if (y) { Py_INCREF(a[7]); return a[7]; }
+        return THPVariable_Wrap(out);
+    });
+}
+
+// bind(device, addresses of the entry points in the order of Entries)
 PyObject* py_bind(PyObject*, PyObject* args) {
     int dev;
-    unsigned long long p[6];
-    if (!PyArg_ParseTuple(args, "iKKKKKK", &dev, &p[0], &p[1], &p[2], &p[3], &p[4], &p[5])) return nullptr;
+    unsigned long long p[12];
+    if (!PyArg_ParseTuple(args, "iKKKKKKKKKKKK", &dev, &p[0], &p[1], &p[2], &p[3], &p[4], &p[5], &p[6], &p[7], &p[8], &p[9], &p[10], &p[11])) return nullptr;
     g.gemm = reinterpret_cast<decltype(g.gemm)>(p[0]);
     g.gemm_multi = reinterpret_cast<decltype(g.gemm_multi)>(p[1]);
     g.moe_gemv = reinterpret_cast<decltype(g.moe_gemv)>(p[2]);
     g.lm_head = reinterpret_cast<decltype(g.lm_head)>(p[3]);
     g.moe_route = reinterpret_cast<decltype(g.moe_route)>(p[4]);
     g.moe_ffn = reinterpret_cast<decltype(g.moe_ffn)>(p[5]);
+    g.dequantize = reinterpret_cast<decltype(g.dequantize)>(p[6]);
+    g.mxfp4_quantize = reinterpret_cast<decltype(g.mxfp4_quantize)>(p[7]);
+    g.mxfp4_packed_size = reinterpret_cast<decltype(g.mxfp4_packed_size)>(p[8]);
+    g.mxfp4_workspace_size = reinterpret_cast<decltype(g.mxfp4_workspace_size)>(p[9]);
+    g.mxfp4_gemm = reinterpret_cast<decltype(g.mxfp4_gemm)>(p[10]);
+    g.mxfp4_moe_grouped = reinterpret_cast<decltype(g.mxfp4_moe_grouped)>(p[11]);
     g_device = dev;
     Py_RETURN_NONE;
 }
 
 #define LP_FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_##name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {LP_FAST(gemm), LP_FAST(gemm_multi), LP_FAST(moe_gemv), LP_FAST(lm_head), LP_FAST(moe_route), LP_FAST(moe_ffn),
+PyMethodDef methods[] = {LP_FAST(gemm), LP_FAST(gemm_multi), LP_FAST(moe_gemv), LP_FAST(lm_head), LP_FAST(moe_route), LP_FAST(moe_ffn), LP_FAST(dequantize), LP_FAST(mxfp4_quantize), LP_FAST(mxfp4_gemm), LP_FAST(mxfp4_moe_grouped),
                          {"bind", py_bind, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

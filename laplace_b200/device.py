@@ -37,7 +37,8 @@ def lib(device: int | None = None):
             n = None
         if n is not None:
             n.bind(dev, *(ctypes.cast(getattr(L, "laplace_cuda_" + f), ctypes.c_void_p).value
-                          for f in ("gemm_dev", "gemm_multi_dev", "moe_gemv_dev", "lm_head_dev", "moe_route_dev", "moe_ffn_dev")))
+                          for f in ("gemm_dev", "gemm_multi_dev", "moe_gemv_dev", "lm_head_dev", "moe_route_dev", "moe_ffn_dev", "dequantize_dev", "mxfp4_quantize_dev",
+                                    "mxfp4_packed_size", "mxfp4_workspace_size", "mxfp4_gemm_dev", "mxfp4_moe_grouped_dev")))
         _native = n
         _ready_on = dev
         from . import matmul as _m
@@ -222,6 +223,9 @@ def debug_blocksums(x: torch.Tensor, w: torch.Tensor, t: int, M: int, K: int, N:
 
 def dequantize(w: torch.Tensor, t: int, n: int) -> torch.Tensor:
     """dequantize(w, dst, n) of src/matmul.cpp:504 on device blocks."""
+    r = _native and _native.dequantize(w, t, n)
+    if r is not None:
+        return r
     dst = torch.empty(n, dtype=torch.float32, device=w.device)
     L = lib()
     _check(L, L.laplace_cuda_dequantize_dev(w.data_ptr(), int(t), dst.data_ptr(), n, _stream()))
@@ -258,6 +262,9 @@ def _here(*tensors) -> bool:
 def mxfp4_quantize(x: torch.Tensor, w: torch.Tensor | None = None) -> torch.Tensor:
     """Values (fp32, fp16 or bf16; rows a multiple of 32 long) -> MXFP4 blocks as GGUF holds them, flat bytes
     (laplace_cuda_mxfp4_quantize_dev). dequantize, embed_rows and mxfp4_pack take them."""
+    r = _native.mxfp4_quantize(x) if _native and w is None else None
+    if r is not None:
+        return r
     L = lib()
     assert x.dtype in _MX_FLOATS and _here(x, w) and x.dim() >= 1 and x.shape[-1] % 32 == 0
     n = x.numel()
@@ -280,6 +287,9 @@ def mxfp4_pack(w: torch.Tensor, N: int, K: int, n_experts: int = 1) -> torch.Ten
 
 def mxfp4_gemm(x: torch.Tensor, packed: torch.Tensor, M: int, K: int, N: int, y: torch.Tensor | None = None) -> torch.Tensor:
     """y[m] = W . x[m] with packed MXFP4 weights and x quantized to MXFP8 (laplace_cuda_mxfp4_gemm_dev)."""
+    r = _native and _native.mxfp4_gemm(x, packed, M, K, N, y)
+    if r is not None:
+        return r
     L = lib()
     assert x.dtype == torch.float32 and packed.dtype == torch.uint8 and _here(x, packed, y) and M >= 0 and x.numel() >= M * K
     assert packed.numel() >= L.laplace_cuda_mxfp4_packed_size(1, N, K)
@@ -295,6 +305,9 @@ def mxfp4_moe_grouped(x: torch.Tensor, packed: torch.Tensor, pair_expert: torch.
                       n_experts_total: int, K: int, N: int, y: torch.Tensor | None = None) -> torch.Tensor:
     """y[p] = W[pair_expert[p]] . x[pair_row[p]] for (token, expert) pairs in any order, as moe_grouped, with packed MXFP4
     experts (laplace_cuda_mxfp4_moe_grouped_dev). pair_row None: pair p reads row p. A negative expert leaves its row of y as it was."""
+    r = _native and _native.mxfp4_moe_grouped(x, packed, pair_expert, pair_row, n_experts_total, K, N, y)
+    if r is not None:
+        return r
     L = lib()
     P = pair_expert.numel()
     assert K > 0 and pair_expert.dtype == torch.int32 and (pair_row is None or (pair_row.dtype == torch.int32 and pair_row.numel() == P))

@@ -419,3 +419,30 @@ def test_expert_layer_and_head():
     _close(h, *_grouped_ref(x, gu_v.reshape(E, 2 * I, H), e, row.cpu().numpy(), np.zeros((T * k, 2 * I))), H, "gate / up")
     _close(d, *_grouped_ref(act.cpu().numpy(), dn_v.reshape(E, H, I), e, None, np.zeros((T * k, H))), I, "down")
     _close(logits, *ref.product(out.cpu().numpy(), head_v.reshape(V, H)), H, "head")
+
+
+def test_native_and_general_paths_agree():
+    import torch
+    from laplace_b200 import device
+    device.lib()
+    assert device._native is not None
+    w, _ = _blocks(1200, 64, 96)
+    calls = _calls(1210) + [lambda: device.dequantize(_dev(w), MX, 64 * 96)]
+    native = device._native
+    fast = [f() for f in calls]
+    try:
+        device._native = None
+        slow = [f() for f in calls]
+    finally:
+        device._native = native
+    assert all(torch.equal(a, b) and a.dtype == b.dtype and a.shape == b.shape for a, b in zip(fast, slow))
+    x = _dev(_act(1220, 2, 96))
+    p = device.mxfp4_pack(_dev(w), 64, 96)
+    for bad in (lambda v: device.mxfp4_gemm(v, p, 1, 96, 64), lambda v: device.mxfp4_quantize(v.reshape(1, -1)),
+                lambda v: device.mxfp4_moe_grouped(v, p, torch.zeros(1, dtype=torch.int32, device="cuda"), None, 1, 96, 64)):
+        def f(v):                                               # inside a transform tensors have no storage
+            with pytest.raises(RuntimeError):
+                bad(v)
+            return v.sum()
+        torch.vmap(f)(x)
+    device.sync()
