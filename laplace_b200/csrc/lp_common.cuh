@@ -117,6 +117,7 @@ int launch_gemm_f32act(const float* x, const uint8_t* w, uint32_t type, float* y
 int launch_dequantize(const uint8_t* w, uint32_t type, float* dst, long long n, float scale, cudaStream_t st);
 int launch_embed_rows(const uint8_t* w, uint32_t type, const int* tokens, int M, int H, long long vocab, float scale, float* dst,
                       cudaStream_t st);
+int launch_mxfp4_dequantize(const uint8_t* w, float* dst, long long n, cudaStream_t st);      // lp_mx.cu
 int launch_softcap(float* y, long long n, float cap, cudaStream_t st);
 int launch_allgather_wait(const PeerOut& po, cudaStream_t st, bool advance = false);
 int launch_gemm_sa_multi(const float* x, const float* norm_w, float eps, float* x_norm_out, const uint8_t* const* ws, float* const* ys,

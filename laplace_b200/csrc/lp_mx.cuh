@@ -40,6 +40,12 @@ __device__ __forceinline__ uint32_t e2m1x2(float a, float b) {
     asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n\tcvt.u32.u8 %0, t;\n\t}" : "=r"(r) : "f"(a), "f"(b));
     return r;
 }
+// the values of two e2m1 codes
+__device__ __forceinline__ float2 e2m1x2_value(uint32_t c) {
+    uint32_t h;
+    asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(h) : "r"(c));
+    return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
 // four values as e4m3, the first in the lowest byte
 __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
     uint16_t lo, hi;

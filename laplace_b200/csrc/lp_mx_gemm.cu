@@ -175,11 +175,10 @@ __global__ void __launch_bounds__(THREADS, 1) mx_gemm_kernel(const __grid_consta
         int it = 0;
         bool ok = true;
         for (int seg = 0; ok && walk(s); ++seg) {
-            const int acc = seg % L::ACCS, n = (s.n + 15) & ~15;
+            const int acc = seg % L::ACCS, n = (s.n + 15) & ~15, groups = (s.n + 127) >> 7;
             const uint32_t d = tmem + acc * NT;
             if (seg >= L::ACCS && !wait_or_abort<true>(sb + L::TEMPTY + 8 * acc, (seg / L::ACCS - 1) & 1, abort_flag, a.err, DEV_TIMEOUT_TMEM)) break;
             fence_after();
-            const int groups = (s.n + 127) >> 7;
             for (int kt = s.k0; kt < s.k1; ++kt, ++it) {
                 const int st = it % L::STAGES;
                 if (!wait_or_abort<true>(sb + L::FULL + 8 * st, (it / L::STAGES) & 1, abort_flag, a.err, DEV_TIMEOUT_FULL)) { ok = false; break; }

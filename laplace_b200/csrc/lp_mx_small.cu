@@ -20,7 +20,7 @@ using namespace mx;
 using namespace tc;
 
 constexpr int THREADS = 320;
-constexpr int QUANT = 4;                       // quantizer warps
+constexpr int QUANT = 4;                       // quantizer warps. At most the stages: a warp that waits for a stage must have seen the use before the last one end
 constexpr int TOK = 8, MAX_PAIRS = 32;
 constexpr int N_MMA = 16;                      // columns of the instruction; those from TOK on are not read
 constexpr int ACCS = 8;                        // accumulators in TMEM
@@ -55,7 +55,7 @@ __device__ __forceinline__ void arrive_release(uint32_t remote_bar) { asm volati
 __device__ __forceinline__ void st_cluster(uint32_t addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" :: "r"(addr), "f"(v) : "memory"); }
 
 template <int C, bool GROUPED>
-__global__ void __launch_bounds__(THREADS, 1) mx_small_kernel(const __grid_constant__ CUtensorMap map, const SmallArgs a) {
+__global__ void __launch_bounds__(THREADS, 2) mx_small_kernel(const __grid_constant__ CUtensorMap map, const SmallArgs a) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t sb = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem = smem_raw + (sb - smem_u32(smem_raw));
@@ -206,6 +206,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx_small_kernel(const __grid_const
         const int r = threadIdx.x - 128;                // weight row of the tile
         const uint32_t quadrant = static_cast<uint32_t>(warp & 3) * 32u << 16;
         asm volatile("griddepcontrol.wait;" ::: "memory");
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
         if (C > 1) cluster_wait();
         int i = 0;
         for (int t = cluster; t < tiles; t += clusters, ++i) {
@@ -264,7 +265,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx_small_kernel(const __grid_const
     }
 }
 
-constexpr size_t SMEM = 227 * 1024;
+constexpr size_t SMEM = 113 * 1024;
 int slot_tokens(int M) { return M < TOK ? M : TOK; }
 int stages_of(int C, int M) {
     const size_t left = SMEM - 1024 - sizeof(Fixed) - (C > 1 ? static_cast<size_t>(SLOTS) * C * slot_tokens(M) * 512 : 0);
@@ -281,7 +282,7 @@ int clusters_at_once(cudaLaunchConfig_t cfg) {
         int got = 0;
         n = cudaFuncSetAttribute(mx_small_kernel<C, GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) == cudaSuccess &&
                     (C == 1 || cudaOccupancyMaxActiveClusters(&got, mx_small_kernel<C, GROUPED>, &cfg) == cudaSuccess)
-                ? (C == 1 ? ctx().sm_count : got) : 0;
+                ? (C == 1 ? 2 * ctx().sm_count : got) : 0;
         cudaGetLastError();
     }
     return n;
@@ -319,7 +320,7 @@ int launch_small(const CUtensorMap& map, const SmallArgs& a, int tiles, cudaStre
     long long least = 1ll << 62;
     for (int i = 0; i < 4; ++i) {
         const int c = 1 << i;
-        if (!n[i] || a.kts < c) continue;
+        if (!n[i] || a.kts < c || stages_of(c, a.M) < QUANT) continue;
         const long long steps = static_cast<long long>((tiles + n[i] - 1) / n[i]) * ((a.kts + c - 1) / c) + (c > 1 ? 2 : 0);
         if (steps < least) { least = steps; best = i; }
     }

@@ -605,6 +605,7 @@ int launch_dequantize(const uint8_t* w, uint32_t type, float* dst, long long n, 
     if (!w || !dst || n <= 0 || n % g.elems) return fail(LAPLACE_ERR_ARG, "dequantize: n=%lld is not a positive multiple of %d", n, g.elems);
     if ((reinterpret_cast<uintptr_t>(dst) & 15) || (reinterpret_cast<uintptr_t>(w) & align_mask(type)))
         return fail(LAPLACE_ERR_ARG, "dequantize: dst must be 16-byte aligned, blocks 2-byte (F32: 16-byte, MXFP4: any) aligned");
+    if (type == T_MXFP4 && scale == 1.0f) return launch_mxfp4_dequantize(w, dst, n, st);
     const long long groups = n / 16;
     long long blocks = (groups + 255) / 256;
     if (blocks > static_cast<long long>(ctx().sm_count) * 16) blocks = static_cast<long long>(ctx().sm_count) * 16;
