@@ -183,13 +183,13 @@ __global__ void __launch_bounds__(256) mx_act_kernel(const float* __restrict__ x
 // of an expert begin, so that a pair's place is by its number and not by timing. An expert gets whole groups of 8 rows of the image
 // and token tiles of its own. (A warp per expert walking all pairs: 158 us for 16,384 pairs and 128 experts, 32 of them to a block.)
 __device__ __forceinline__ int pair_expert_of(const int* pair_expert, const int* pair_row, int p, int P, int E, int x_rows) {
-    if (p >= P) return -1;
-    const int e = __ldg(pair_expert + p);
-    if (e < 0) return -1;
-    return e >= E || (pair_row && static_cast<unsigned>(__ldg(pair_row + p)) >= static_cast<unsigned>(x_rows)) ? -2 : e;
+    // no branch, so that the loads of several pairs are under way at once
+    const int q = p < P ? p : P - 1, e = __ldg(pair_expert + q), r = pair_row ? __ldg(pair_row + q) : 0;
+    const bool bad = e >= E || (pair_row && static_cast<unsigned>(r) >= static_cast<unsigned>(x_rows));
+    return p >= P || e < 0 ? -1 : bad ? -2 : e;
 }
 __global__ void __launch_bounds__(1024) mx_group_kernel(const int* __restrict__ pair_expert, const int* __restrict__ pair_row, int P, int E, int x_rows, int tile_w, int tile_groups,
-                                                        int2* __restrict__ place, int* __restrict__ out_row, int4* __restrict__ tab, int* __restrict__ n_tiles, int* err) {
+                                                        int2* __restrict__ place, int* __restrict__ out_row, int4* __restrict__ tab, int4* __restrict__ work, int row_tiles, int nt, int kts, int n, int* err) {
     extern __shared__ int sm[];
     const int W = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int* start = sm;                       // first row of an expert in the image
@@ -241,7 +241,11 @@ __global__ void __launch_bounds__(1024) mx_group_kernel(const int* __restrict__ 
             rows += __shfl_sync(0xffffffffu, ri, 31);
             tiles += __shfl_sync(0xffffffffu, ti, 31);
         }
-        if (lane == 0) *n_tiles = tiles;
+        // how the tiles are shared out (cut_of): a number of parts per lane
+        const int all = tiles * row_tiles, most = most_parts(all, kts, n);
+        const int best = __reduce_min_sync(0xffffffffu, lane < most ? cut_cost(nt, kts, lane + 1) * MAX_PARTS + lane : 0x7fffffff);
+        const Cut c = cut_of(nt, all, kts, n, best % MAX_PARTS + 1, best / MAX_PARTS);
+        if (lane == 0) *work = make_int4(c.tiles, c.cut, c.ctas, 0);
     }
     __syncthreads();
     for (int q = p0; q < p1; q += 32 * U) {
@@ -278,8 +282,8 @@ size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
 // What a call keeps in its workspace, and where.
 struct Plan {
-    int    kts, rts, img_rows, groups, nt, tile_w, tile_groups, tiles_m, max_tiles, n_counters;
-    size_t img, sf, counters, part, place, out_row, tab, n_tiles, bytes;
+    int    kts, rts, row_tiles, img_rows, groups, nt, tile_w, tile_groups, tiles_m, max_tiles, n_counters;
+    size_t img, sf, counters, part, place, out_row, tab, work, bytes;
 };
 Plan plan_of(int rows, int experts, int K, int N) {
     Plan p{};
@@ -290,8 +294,10 @@ Plan plan_of(int rows, int experts, int K, int N) {
     const int per = experts ? (rows + experts - 1) / experts : rows;
     p.nt = per <= 32 ? 32 : per <= 64 ? 64 : per <= 128 ? 128 : 256;
     p.tiles_m = (rows + p.nt - 1) / p.nt;
+    const int cg = mx_gemm_cg(p.nt);
+    p.row_tiles = (p.rts + cg - 1) / cg;
     p.tile_w = experts ? p.nt : ((rows + p.tiles_m - 1) / p.tiles_m + 31) & ~31;
-    p.n_counters = ctx().sm_count;
+    p.n_counters = mx_gemm_counters();
     p.tile_groups = (p.nt + 127) / 128;
     p.max_tiles = experts ? rows / p.tile_w + (experts < rows ? experts : rows) : p.tiles_m;
     p.groups = p.max_tiles * p.tile_groups;
@@ -300,12 +306,12 @@ Plan plan_of(int rows, int experts, int K, int N) {
     p.img = take(static_cast<size_t>(p.kts) * p.img_rows * 128);
     p.sf = take(static_cast<size_t>(p.kts) * p.groups * SF_TILE);
     p.counters = take(p.n_counters * sizeof(unsigned));
-    p.part = take(mx_gemm_part_bytes(p.nt, experts ? ctx().sm_count : static_cast<int>(static_cast<long long>(p.tiles_m) * p.rts % ctx().sm_count)));
+    p.part = take(mx_gemm_part_bytes(p.nt));
     if (experts) {
         p.place = take(static_cast<size_t>(rows) * sizeof(int2));
         p.out_row = take(static_cast<size_t>(p.img_rows) * 4);
         p.tab = take(static_cast<size_t>(p.max_tiles) * sizeof(int4));
-        p.n_tiles = take(4);
+        p.work = take(sizeof(int4));
     }
     p.bytes = at;
     return p;
@@ -321,15 +327,16 @@ int launch_product(const float* x, int x_rows, const uint8_t* packed, const int*
     a.q = packed;
     a.sfa = packed + static_cast<size_t>(GROUPED ? experts : 1) * p.rts * p.kts * Q_TILE;
     a.img = ws + p.img; a.sfb = ws + p.sf; a.y = y;
-    a.M = rows; a.N = N; a.kts = p.kts; a.rts = p.rts; a.img_rows = p.img_rows; a.groups = p.groups; a.tile_w = p.tile_w; a.tiles_m = p.tiles_m; a.tile_groups = p.tile_groups;
+    a.M = rows; a.N = N; a.kts = p.kts; a.rts = p.rts; a.img_rows = p.img_rows; a.groups = p.groups; a.tile_w = p.tile_w; a.tiles_m = p.tiles_m; a.tile_groups = p.tile_groups; a.row_tiles = p.row_tiles;
     a.part = reinterpret_cast<float*>(ws + p.part); a.counters = reinterpret_cast<unsigned*>(ws + p.counters); a.err = c.d_err;
     int2* place = nullptr;
+    const int units = c.sm_count / mx_gemm_cg(p.nt);
     int rc;
     if (GROUPED) {
         place = reinterpret_cast<int2*>(ws + p.place);
         a.out_row = reinterpret_cast<int*>(ws + p.out_row);
         a.tab = reinterpret_cast<int4*>(ws + p.tab);
-        a.n_tiles = reinterpret_cast<int*>(ws + p.n_tiles);
+        a.work = reinterpret_cast<int4*>(ws + p.work);
         const int warps = group_warps(experts);
         static bool configured = false;
         if (!configured) {
@@ -337,9 +344,16 @@ int launch_product(const float* x, int x_rows, const uint8_t* packed, const int*
             configured = true;
         }
         rc = launch_early(mx_group_kernel, dim3(1), warps * 32, (warps + 2) * static_cast<size_t>(experts) * sizeof(int), st, pair_expert, pair_row, rows, experts, x_rows, p.tile_w,
-                          p.tile_groups, place, reinterpret_cast<int*>(ws + p.out_row), reinterpret_cast<int4*>(ws + p.tab), reinterpret_cast<int*>(ws + p.n_tiles), c.d_err);
+                          p.tile_groups, place, reinterpret_cast<int*>(ws + p.out_row), reinterpret_cast<int4*>(ws + p.tab), reinterpret_cast<int4*>(ws + p.work), p.row_tiles, p.nt, p.kts, units, c.d_err);
         c.launches++;
         if (rc) return rc;
+    }
+    if (!GROUPED) {
+        const int tiles = p.tiles_m * p.row_tiles, most = most_parts(tiles, p.kts, units);
+        int parts = 1;
+        for (int q = 2; q <= most; ++q)
+            if (cut_cost(p.nt, p.kts, q) < cut_cost(p.nt, p.kts, parts)) parts = q;
+        a.dense = cut_of(p.nt, tiles, p.kts, units, parts, cut_cost(p.nt, p.kts, parts));
     }
     const long long warps = static_cast<long long>(rows) * ((p.kts + 1) / 2);
     rc = launch_early(mx_act_kernel<GROUPED>, dim3(static_cast<unsigned>((warps + 7) / 8)), 256, 0, st, x, K, p.kts, rows, ActDst{ws + p.img, ws + p.sf, p.img_rows, p.groups, p.tile_w, p.tile_groups},
@@ -349,6 +363,8 @@ int launch_product(const float* x, int x_rows, const uint8_t* packed, const int*
     return launch_mx_gemm(a, p.nt, static_cast<long long>(GROUPED ? experts : 1) * p.rts * p.kts, GROUPED, st);
 }
 
+// rows: token tiles times row tiles are counted in 32 bits
+bool too_many(long long rows, long long experts, int N) { return (rows / 32 + experts + 1) * ((N + 127) / 128) > 0x3fffffffll; }
 int bad_shape(const char* what, int K, int N, long long experts) {
     if (K <= 0 || N <= 0 || experts <= 0 || K % 32) return fail(LAPLACE_ERR_ARG, "%s: K=%d (a positive multiple of 32) N=%d experts=%lld", what, K, N, experts);
     // rows of 64 bytes that the tensor map of the weights counts
@@ -427,7 +443,7 @@ int laplace_cuda_mxfp4_gemm_dev(const float* x, const uint8_t* packed, float* y,
     if (const int rc = bad_shape("mxfp4_gemm", K, N, 1)) return rc;
     if (M < 0) return fail(LAPLACE_ERR_ARG, "mxfp4_gemm: M=%d", M);
     if (M == 0) return LAPLACE_OK;
-    if (M > 1 << 24) return fail(LAPLACE_ERR_LIMIT, "mxfp4_gemm: M=%d", M);
+    if (M > 1 << 24 || too_many(M, 1, N)) return fail(LAPLACE_ERR_LIMIT, "mxfp4_gemm: M=%d", M);
     if (!x || !packed || !y || !workspace) return fail(LAPLACE_ERR_ARG, "mxfp4_gemm: null pointer");
     if (misaligned(x, 16) || misaligned(packed, 128) || misaligned(workspace, 256) || misaligned(y, 4))
         return fail(LAPLACE_ERR_ARG, "mxfp4_gemm: x must be 16-byte, packed 128-byte, workspace 256-byte aligned");
@@ -441,7 +457,7 @@ int laplace_cuda_mxfp4_moe_grouped_dev(const float* x, int x_rows, const uint8_t
     if (const int rc = bad_shape("mxfp4_moe_grouped", K, N, n_experts_total)) return rc;
     if (n_pairs < 0 || x_rows < 0) return fail(LAPLACE_ERR_ARG, "mxfp4_moe_grouped: n_pairs=%d x_rows=%d", n_pairs, x_rows);
     if (n_pairs == 0) return LAPLACE_OK;
-    if (n_pairs > 1 << 24) return fail(LAPLACE_ERR_LIMIT, "mxfp4_moe_grouped: n_pairs=%d", n_pairs);
+    if (n_pairs > 1 << 24 || too_many(n_pairs, n_experts_total, N)) return fail(LAPLACE_ERR_LIMIT, "mxfp4_moe_grouped: n_pairs=%d", n_pairs);
     if (n_experts_total > MAX_EXPERTS) return fail(LAPLACE_ERR_LIMIT, "mxfp4_moe_grouped: %d experts, %d at most", n_experts_total, MAX_EXPERTS);
     if (!x || !packed || !pair_expert || !y || !workspace) return fail(LAPLACE_ERR_ARG, "mxfp4_moe_grouped: null pointer");
     if (!pair_row && x_rows < n_pairs) return fail(LAPLACE_ERR_ARG, "mxfp4_moe_grouped: %d rows of x for %d pairs", x_rows, n_pairs);

@@ -3,10 +3,13 @@
 // Formats and layouts: lp_mx.cu. The instruction takes the 4-bit weights and their scale bytes as they lie in memory: no thread
 // touches a weight. TMA spreads the 8 bytes of 16 values over 16 bytes of shared memory on the way in, the form that the instruction reads.
 //
-// Work. Tiles of 128 weight rows x NT tokens, k in steps of 128. Of T tiles and G CTAs (one per SM) the last T - T % G go to the CTAs
-// one after the other, whole; the T % G before them are cut: their k steps, in tile order, in equal runs to the CTAs. A CTA that has a part
-// of a tile leaves its sums in the workspace; the last of a tile's CTAs to arrive (a counter) adds them up in the order of k, so that the
-// result does not depend on who was last. Few rows (decode) are all cut: every SM streams the same share of the weights.
+// Work. Tiles of 128 weight rows x NT tokens, k in steps of 128, G CTAs (one per SM). Whole tiles go to the CTAs one after the other; the last ones, where
+// they do not come out even, may be cut: their k steps, in tile order, go in equal runs to the CTAs (cut_of in lp_mx.cuh says when that pays). Of a
+// cut tile's CTAs the last one to arrive (a counter) keeps its sums in registers; the others leave theirs in the workspace, on which
+// it waits - they are running, so it does not wait long - and it adds all up in the order of k: the result does not depend on who was last.
+//
+// More than 128 tokens a tile: a pair of SMs (cta_group::2) takes 256 weight rows x 256 tokens, each CTA with its 128 rows and half of the tokens
+// in shared memory. What bounds one CTA with 128 x 256 is the way from L2: 41 KB a step of 512 cycles; a pair's CTAs take 25 KB each.
 //
 // Roles by warp: 0 copies, 1 MMA issue (owns the TMEM), 4-11 drain (lane = weight row). All waits are bounded; a wait that gives up
 // raises the status word and the roles leave their loops.
@@ -25,44 +28,42 @@ constexpr int DRAIN = 256;                     // threads of the drain: two warp
 constexpr int A_STAGE = 128 * 128;             // 128 rows x 128 values, a byte each after the copy
 constexpr uint32_t SF_COL = 480;               // TMEM columns of the scales: two sets of 16 (4 of the weights, up to 8 of the activations)
 
+// CTAs of a tile of NT tokens.
+constexpr int cg_of(int nt) { return nt == 256 ? 2 : 1; }
+
 template <int NT> struct Lay {
+    static constexpr int CG = cg_of(NT), B_STAGE = NT / CG * 128;
     static constexpr int GROUPS = (NT + 127) / 128;       // 128-row groups of scales
-    static constexpr int STAGE = A_STAGE + NT * 128 + SF_TILE + GROUPS * SF_TILE;
+    static constexpr int STAGE = A_STAGE + B_STAGE + SF_TILE + GROUPS * SF_TILE;
     static constexpr int STAGES = (226 * 1024 - 1024) / STAGE;
     static constexpr int ACCS = NT == 256 ? 1 : 2;
-    static constexpr uint32_t A = 0, B = A + STAGES * A_STAGE, SFA = B + STAGES * NT * 128, SFB = SFA + STAGES * SF_TILE, BAR = SFB + STAGES * GROUPS * SF_TILE;
-    static constexpr uint32_t FULL = BAR, EMPTY = FULL + 8 * STAGES, TFULL = EMPTY + 8 * STAGES, TEMPTY = TFULL + 16, PTR = TEMPTY + 16, ABORT = PTR + 4, LAST = ABORT + 4,
-                              BYTES = LAST + 8 + 1024;
+    static constexpr uint32_t A = 0, B = A + STAGES * A_STAGE, SFA = B + STAGES * B_STAGE, SFB = SFA + STAGES * SF_TILE, BAR = SFB + STAGES * GROUPS * SF_TILE;
+    static constexpr uint32_t FULL = BAR, EMPTY = FULL + 8 * STAGES, TFULL = EMPTY + 8 * STAGES, TEMPTY = TFULL + 16, PTR = TEMPTY + 16, ABORT = PTR + 4, SAY = ABORT + 4,
+                              BYTES = SAY + 8 + 1024;
     static_assert(BYTES <= 227 * 1024, "shared memory");
     static_assert(ACCS * NT <= SF_COL, "TMEM columns");
 };
 
+// rt: row tile, of 128 or (pairs) 256 rows
 struct Seg { int expert, rt, row0, n, group, k0, k1, cut; };      // group: first 128-row group of its scales; cut: number of the cut tile, -1 for a whole one
 struct Work { int tiles, cut, ctas; long long units; };
 
-__host__ __device__ __forceinline__ Work work_of(long long tiles, int kts, int grid) {
-    Work w;
-    w.tiles = static_cast<int>(tiles);
-    w.cut = w.tiles % grid;
-    w.units = static_cast<long long>(w.cut) * kts;
-    const long long most = w.units / MIN_STEPS;
-    w.ctas = most < 1 ? (w.units ? 1 : 0) : most < grid ? static_cast<int>(most) : grid;
-    return w;
-}
 __device__ __forceinline__ long long cut_start(const Work& w, int c) { return w.units * c / w.ctas; }
-// the CTA whose run holds unit u
+// the unit whose run holds step u
 __device__ __forceinline__ int cut_owner(const Work& w, long long u) {
     int c = static_cast<int>(u * w.ctas / w.units);
     while (c + 1 < w.ctas && cut_start(w, c + 1) <= u) ++c;
     while (c > 0 && cut_start(w, c) > u) --c;
     return c;
 }
+// Where a unit leaves its part of a tile: it has at most one that begins inside a tile and one that begins a tile.
+__device__ __forceinline__ int slot_of(int unit, bool begins) { return 2 * unit + begins; }
 
 template <bool GROUPED>
 __device__ __forceinline__ void tile_at(const MxArgs& a, int t, Seg& s) {
     if (GROUPED) {
-        const int4 e = __ldg(a.tab + t / a.rts);
-        s.rt = t % a.rts;
+        const int4 e = __ldg(a.tab + t / a.row_tiles);
+        s.rt = t % a.row_tiles;
         s.expert = e.x; s.row0 = e.y; s.n = e.z; s.group = e.w;
     } else {
         s.rt = t / a.tiles_m;
@@ -72,15 +73,15 @@ __device__ __forceinline__ void tile_at(const MxArgs& a, int t, Seg& s) {
         s.n = min(a.tile_w, a.M - s.row0);
     }
 }
-// A CTA's work piece by piece, in the order in which every role walks it.
-template <bool GROUPED>
+// A unit's work piece by piece, in the order in which every role walks it.
+template <bool GROUPED, int CG>
 struct Walk {
     const MxArgs& a;
     const Work w;
     long long u, u1;
     int next;
     __device__ __forceinline__ Walk(const MxArgs& args, const Work& work) : a(args), w(work) {
-        const int c = blockIdx.x;
+        const int c = blockIdx.x / CG;
         u = c < w.ctas ? cut_start(w, c) : 0;
         u1 = c < w.ctas ? cut_start(w, c + 1) : 0;
         next = w.cut + c;
@@ -99,64 +100,95 @@ struct Walk {
         if (next >= w.tiles) return false;
         tile_at<GROUPED>(a, next, s);
         s.k0 = 0; s.k1 = a.kts; s.cut = -1;
-        next += gridDim.x;
+        next += gridDim.x / CG;
         return true;
     }
 };
 
+// Whether any thread of the barrier's says so; all of them learn the same.
+template <int THREADS>
+__device__ __forceinline__ bool any_of(int bar, bool mine) {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(r) : "r"(static_cast<uint32_t>(mine)), "r"(bar), "n"(THREADS) : "memory");
+    return r != 0;
+}
+
 template <int NT, bool GROUPED>
 __global__ void __launch_bounds__(THREADS, 1) mx_gemm_kernel(const __grid_constant__ CUtensorMap map, const MxArgs a) {
     using L = Lay<NT>;
+    constexpr int CG = L::CG;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t sb = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem = smem_raw + (sb - smem_u32(smem_raw));
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::ABORT);
-    const int warp = threadIdx.x >> 5;
+    const int warp = threadIdx.x >> 5, rank = CG == 2 ? static_cast<int>(pair_rank()) : 0;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < L::STAGES; ++i) { mbar_init(sb + L::FULL + 8 * i, 1); mbar_init(sb + L::EMPTY + 8 * i, 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(sb + L::TFULL + 8 * i, 1); mbar_init(sb + L::TEMPTY + 8 * i, DRAIN / 32); }
+        for (int i = 0; i < L::STAGES; ++i) { mbar_init(sb + L::FULL + 8 * i, CG - rank); mbar_init(sb + L::EMPTY + 8 * i, 1); }      // the even CTA's: its own copies and word of the other's
+        for (int i = 0; i < 2; ++i) { mbar_init(sb + L::TFULL + 8 * i, 1); mbar_init(sb + L::TEMPTY + 8 * i, CG * DRAIN / 32); }
         *abort_flag = 0;
         fence_barrier_init();
         asm volatile("prefetch.tensormap [%0];" :: "l"(&map) : "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(sb + L::PTR), "r"(512u) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if constexpr (CG == 2) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(sb + L::PTR), "r"(512u) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(sb + L::PTR), "r"(512u) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     fence_before();
     __syncthreads();
+    if constexpr (CG == 2) {                       // both CTAs' barriers are there before either arrives on them
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
     fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + L::PTR);
     // Experts: the table of token tiles is made by the kernels before this one. One matrix: the weights may be copied meanwhile; the quantizer
     // before this kernel lets it start only after it has itself waited for what is before it in the stream, weights' writers included.
     if (GROUPED || warp != 0) asm volatile("griddepcontrol.wait;" ::: "memory");
-    const Work w = work_of(GROUPED ? static_cast<long long>(*a.n_tiles) * a.rts : static_cast<long long>(a.tiles_m) * a.rts, a.kts, gridDim.x);
+    const int3 cut = GROUPED ? make_int3(a.work->x, a.work->y, a.work->z) : make_int3(a.dense.tiles, a.dense.cut, a.dense.ctas);
+    const Work w{cut.x, cut.y, cut.z, static_cast<long long>(cut.y) * a.kts};
 
+    if (warp < 4) {
+    if constexpr (NT == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");       // 128 x 64 + 256 x 216 of 384 x 168 registers
     if (warp == 0 && elect_one()) {
-        auto tile_of = [&](const Seg& s, int kt) { return (static_cast<size_t>(s.expert) * a.rts + s.rt) * a.kts + kt; };
+        // of this CTA: its row tile (of an odd number the last one twice, the second time for nothing), its part of the tokens
+        auto tile_of = [&](const Seg& s, int kt) { return (static_cast<size_t>(s.expert) * a.rts + min(s.rt * CG + rank, a.rts - 1)) * a.kts + kt; };
+        auto rows_of = [&](const Seg& s, int& first) {
+            const int n8 = (s.n + 7) & ~7, half = ((s.n + 31) & ~31) / 2;
+            if (CG == 1) { first = 0; return n8; }
+            first = rank * half;
+            return rank ? max(n8 - half, 0) : min(n8, half);
+        };
         auto weights = [&](int st, const Seg& s, int kt) {
-            const int n8 = (s.n + 7) & ~7, groups = (s.n + 127) >> 7;
+            int first;
+            const int groups = (s.n + 127) >> 7;
             const uint32_t bar = sb + L::FULL + 8 * st;
-            mbar_expect_tx(bar, Q_TILE + SF_TILE + n8 * 128 + groups * SF_TILE);
+            mbar_expect_tx(bar, Q_TILE + SF_TILE + rows_of(s, first) * 128 + groups * SF_TILE);
             const size_t tile = tile_of(s, kt);
             tma_load_2d(sb + L::A + st * A_STAGE, &map, 0, static_cast<int>(tile * 128), bar);
             bulk_g2s(sb + L::SFA + st * SF_TILE, a.sfa + tile * SF_TILE, SF_TILE, bar);
         };
         auto tokens = [&](int st, const Seg& s, int kt) {
-            const int n8 = (s.n + 7) & ~7, groups = (s.n + 127) >> 7;
+            int first;
+            const int rows = rows_of(s, first), groups = (s.n + 127) >> 7;
             const uint32_t bar = sb + L::FULL + 8 * st;
-            bulk_g2s(sb + L::B + st * NT * 128, a.img + (static_cast<size_t>(kt) * a.img_rows + s.row0) * 128, n8 * 128, bar);
+            if (rows) bulk_g2s(sb + L::B + st * L::B_STAGE, a.img + (static_cast<size_t>(kt) * a.img_rows + s.row0 + first) * 128, rows * 128, bar);
             bulk_g2s(sb + L::SFB + st * L::GROUPS * SF_TILE, a.sfb + (static_cast<size_t>(kt) * a.groups + s.group) * SF_TILE, groups * SF_TILE, bar);
         };
         int early = 0;
         if (!GROUPED) {
-            Walk<GROUPED> walk(a, w);
+            Walk<GROUPED, CG> walk(a, w);
             Seg s;
             while (early < L::STAGES && walk(s))
                 for (int kt = s.k0; kt < s.k1 && early < L::STAGES; ++kt) weights(early++, s, kt);
             asm volatile("griddepcontrol.wait;" ::: "memory");
         }
-        Walk<GROUPED> walk(a, w);
+        Walk<GROUPED, CG> walk(a, w);
         Seg s;
         int it = 0;
         bool ok = true;
@@ -169,133 +201,174 @@ __global__ void __launch_bounds__(THREADS, 1) mx_gemm_kernel(const __grid_consta
             }
         if (!ok)                                        // what is in flight lands before the CTA goes
             for (int i = 0; i < 1000; ++i) __nanosleep(1000);
-    } else if (warp == 1 && elect_one()) {
-        Walk<GROUPED> walk(a, w);
+    } else if (warp == 1 && rank == 0 && elect_one()) {
+        Walk<GROUPED, CG> walk(a, w);
         Seg s;
         int it = 0;
         bool ok = true;
+        auto wait = [&](uint32_t bar, int parity, int code) {
+            return CG == 2 ? wait_pair(bar, parity, abort_flag, a.err, code) : wait_or_abort<true>(bar, parity, abort_flag, a.err, code);
+        };
+        auto done = [&](uint32_t bar) {
+            if constexpr (CG == 2) commit_pair(bar);
+            else commit(bar);
+        };
         for (int seg = 0; ok && walk(s); ++seg) {
-            const int acc = seg % L::ACCS, n = (s.n + 15) & ~15, groups = (s.n + 127) >> 7;
+            const int acc = seg % L::ACCS, n = CG == 2 ? (s.n + 31) & ~31 : (s.n + 15) & ~15, groups = (s.n + 127) >> 7;
             const uint32_t d = tmem + acc * NT;
-            if (seg >= L::ACCS && !wait_or_abort<true>(sb + L::TEMPTY + 8 * acc, (seg / L::ACCS - 1) & 1, abort_flag, a.err, DEV_TIMEOUT_TMEM)) break;
+            if (seg >= L::ACCS && !wait(sb + L::TEMPTY + 8 * acc, (seg / L::ACCS - 1) & 1, DEV_TIMEOUT_TMEM)) { ok = false; break; }
             fence_after();
             for (int kt = s.k0; kt < s.k1; ++kt, ++it) {
                 const int st = it % L::STAGES;
-                if (!wait_or_abort<true>(sb + L::FULL + 8 * st, (it / L::STAGES) & 1, abort_flag, a.err, DEV_TIMEOUT_FULL)) { ok = false; break; }
+                if (!wait(sb + L::FULL + 8 * st, (it / L::STAGES) & 1, DEV_TIMEOUT_FULL)) { ok = false; break; }
                 fence_after();
                 const uint32_t sfa = tmem + SF_COL + 16 * (it & 1), sfb = sfa + 4;
-                copy_scales(sfa, sb + L::SFA + st * SF_TILE);
-                for (int g = 0; g < groups; ++g) copy_scales(sfb + 4 * g, sb + L::SFB + (st * L::GROUPS + g) * SF_TILE);
-                const uint64_t ad = smem_desc_sw128(sb + L::A + st * A_STAGE), bd = smem_desc_sw128(sb + L::B + st * NT * 128);
+                copy_scales<CG>(sfa, sb + L::SFA + st * SF_TILE);
+                for (int g = 0; g < groups; ++g) copy_scales<CG>(sfb + 4 * g, sb + L::SFB + (st * L::GROUPS + g) * SF_TILE);
+                const uint64_t ad = smem_desc_sw128(sb + L::A + st * A_STAGE), bd = smem_desc_sw128(sb + L::B + st * L::B_STAGE);
 #pragma unroll
-                for (int ks = 0; ks < 4; ++ks) mma_mx(d, ad + 2 * ks, bd + 2 * ks, idesc_mx(n, ks), sfa, sfb, kt != s.k0 || ks);
-                commit(sb + L::EMPTY + 8 * st);
+                for (int ks = 0; ks < 4; ++ks) mma_mx<CG>(d, ad + 2 * ks, bd + 2 * ks, idesc_mx<CG>(n, ks), sfa, sfb, kt != s.k0 || ks);
+                done(sb + L::EMPTY + 8 * st);
             }
-            if (ok) commit(sb + L::TFULL + 8 * acc);
+            if (ok) done(sb + L::TFULL + 8 * acc);
         }
-    } else if (warp >= 4) {
-        Walk<GROUPED> walk(a, w);
+        if (!ok)                                        // what has been issued ends before the CTA goes
+            for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+    } else if (CG == 2 && warp == 1 && rank == 1 && elect_one()) {      // (elect takes the whole warp: no lane of the even CTA's may come here)
+        // the odd CTA: tells the even one of its stages as they fill
+        Walk<GROUPED, CG> walk(a, w);
+        Seg s;
+        int it = 0;
+        bool ok = true;
+        while (ok && walk(s))
+            for (int kt = s.k0; kt < s.k1; ++kt, ++it) {
+                const int st = it % L::STAGES;
+                if (!wait_or_abort<true>(sb + L::FULL + 8 * st, (it / L::STAGES) & 1, abort_flag, a.err, DEV_TIMEOUT_FULL)) { ok = false; break; }
+                arrive_cluster(map_to_rank(sb + L::FULL + 8 * st, 0));
+            }
+    }
+    } else {
+        if constexpr (NT == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        Walk<GROUPED, CG> walk(a, w);
         Seg s;
         const int lane = threadIdx.x & 31, id = threadIdx.x - 128, half = id >> 7, r = id & 127;      // r: weight row of the tile
         const uint32_t quadrant = static_cast<uint32_t>(warp & 3) * 32u << 16;
-        volatile int* last = reinterpret_cast<volatile int*>(smem + L::LAST);
+        volatile int* say = reinterpret_cast<volatile int*>(smem + L::SAY);
         for (int seg = 0; walk(s); ++seg) {
             const int acc = seg % L::ACCS;
-            if (!wait_or_abort<false>(sb + L::TFULL + 8 * acc, (seg / L::ACCS) & 1, abort_flag, a.err, DEV_TIMEOUT_MMA)) break;
+            const bool ok = wait_or_abort<false>(sb + L::TFULL + 8 * acc, (seg / L::ACCS) & 1, abort_flag, a.err, DEV_TIMEOUT_MMA);
+            // the warps meet at cut tiles (which come first): they leave together or not at all
+            if (s.cut >= 0 ? any_of<DRAIN>(1, !ok) : !ok) break;
             __syncwarp();
             fence_after();
-            const int col = s.rt * 128 + r;
-            float* part = a.part + static_cast<size_t>(blockIdx.x + max(s.cut, 0)) * (NT * 128) + r;
-            for (int c0 = 32 * half; c0 < s.n; c0 += 64) {
-                float v[32];
-                const int here = min(32, s.n - c0);
-                int to = 0;                             // lane: the row of y that column c0 + lane goes to
-                if (GROUPED && s.cut < 0 && lane < here) to = __ldg(a.out_row + s.row0 + c0 + lane);
-                __syncwarp();
-                ld32(tmem + quadrant + acc * NT + c0, v);
-                wait_ld();
-                if (s.cut >= 0) {
-                    float* q = part + c0 * 128;
-                    if (here == 32) {
+            const int rt = s.rt * CG + rank, col = rt * 128 + r, unit = blockIdx.x / CG;
+            // Columns 32 half + 64 j .. + 31: all into registers first, so that the next tile's products do not wait for what follows.
+            constexpr int J = NT < 64 ? 1 : NT / 64;
+            float v[J][32];
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) __stcg(q + i * 128, v[i]);
-                    } else {
+            for (int j = 0; j < J; ++j)
+                if (32 * half + 64 * j < s.n) ld32(tmem + quadrant + acc * NT + 32 * half + 64 * j, v[j]);
+            wait_ld();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (rank == 0) mbar_arrive(sb + L::TEMPTY + 8 * acc);
+                else arrive_cluster(map_to_rank(sb + L::TEMPTY + 8 * acc, 0));
+            }
+            const int full = half ? max(0, s.n - 32) : s.n;      // (columns of the tile from this half's first on)
+            if (s.cut >= 0) {
+                const long long u = static_cast<long long>(s.cut) * a.kts;
+                const int first = cut_owner(w, u), pieces = cut_owner(w, u + a.kts - 1) - first + 1;
+                unsigned* count = a.counters + 2 * (s.cut * CG + rank);      // {arrived, written}
+                auto part = [&](int c, bool begins) { return a.part + static_cast<size_t>(slot_of(c, begins) * CG + rank) * (NT * 128) + half * (32 * 128) + r; };
+                if (id == 0) *say = atomicAdd(count, 1u) == static_cast<unsigned>(pieces - 1);
+                named_bar_sync(1, DRAIN);
+                const bool last = *say;
+                if (!last) {
+                    float* q = part(unit, s.k0 == 0);
+#pragma unroll
+                    for (int j = 0; j < J; ++j)
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
-                            if (i < here) __stcg(q + i * 128, v[i]);
+                            if (64 * j + i < full) __stcg(q + (64 * j + i) * 128, v[j][i]);
+                    named_bar_sync(1, DRAIN);
+                    if (id == 0) { __threadfence(); atomicAdd(count + 1, 1u); }
+                    continue;
+                }
+                bool there = true;
+                if (id == 0) {
+                    there = false;
+                    for (int i = 0; i < 1 << 22 && !there; ++i) {
+                        uint32_t c;
+                        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(c) : "l"(count + 1) : "memory");
+                        there = c == static_cast<unsigned>(pieces - 1);
                     }
-                } else if (GROUPED) {
+                    if (!there) { *abort_flag = 1; report_status(a.err, DEV_TIMEOUT_DRAIN); }
+                }
+                if (any_of<DRAIN>(1, !there)) break;
+#pragma unroll
+                for (int b = 0; b < 2 * J; ++b) {            // sixteen columns at a time
+                    const int c0 = 64 * (b / 2) + 16 * (b % 2);
+                    if (c0 >= full) break;
+                    float sum[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sum[i] = 0.f;
+#pragma unroll 1
+                    for (int p = 0; p < pieces; ++p) {
+                        if (first + p == unit) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) sum[i] += v[b / 2][16 * (b % 2) + i];
+                        } else {
+                            const float* q = part(first + p, p == 0) + c0 * 128;
+                            float o[16];
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o[i] = c0 + i < full ? __ldcg(q + i * 128) : 0.f;
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) sum[i] += o[i];
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[b / 2][16 * (b % 2) + i] = sum[i];
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int c0 = 32 * half + 64 * j, here = min(32, s.n - c0);
+                if (here <= 0) break;
+                if (GROUPED) {
+                    // lane: the row of y that column c0 + lane goes to
+                    const int to = lane < here ? __ldg(a.out_row + s.row0 + c0 + lane) : 0;
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         const int m = __shfl_sync(0xffffffffu, to, i);
-                        if (i < here && col < a.N) a.y[static_cast<size_t>(m) * a.N + col] = v[i];
+                        if (i < here && col < a.N) a.y[static_cast<size_t>(m) * a.N + col] = v[j][i];
                     }
-                } else {
+                } else if (col < a.N) {
                     float* q = a.y + static_cast<size_t>(s.row0 + c0) * a.N + col;
-                    if (here == 32 && col < a.N) {
+                    if (here == 32) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) q[static_cast<size_t>(i) * a.N] = v[i];
-                    } else if (col < a.N) {
+                        for (int i = 0; i < 32; ++i) q[static_cast<size_t>(i) * a.N] = v[j][i];
+                    } else {
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
-                            if (i < here) q[static_cast<size_t>(i) * a.N] = v[i];
+                            if (i < here) q[static_cast<size_t>(i) * a.N] = v[j][i];
                     }
                 }
-            }
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(sb + L::TEMPTY + 8 * acc);
-            if (s.cut < 0) continue;
-            const long long u = static_cast<long long>(s.cut) * a.kts;
-            const int first = cut_owner(w, u), pieces = cut_owner(w, u + a.kts - 1) - first + 1;
-            __threadfence();
-            named_bar_sync(1, DRAIN);
-            if (id == 0) *last = atomicAdd(a.counters + s.cut, 1u) == static_cast<unsigned>(pieces - 1);
-            named_bar_sync(1, DRAIN);
-            if (!*last) continue;
-            __threadfence();
-            // four rows of a column a thread, eight columns at a time; parts in the order of k
-            const int r4 = (id & 31) * 4, col4 = s.rt * 128 + r4;
-            const float* p0 = a.part + static_cast<size_t>(first + s.cut) * (NT * 128) + r4;
-            const bool vec = (a.N & 3) == 0 && (reinterpret_cast<uintptr_t>(a.y) & 15) == 0;
-            for (int c0 = id >> 5; c0 < s.n; c0 += 32) {
-                float4 sum[4] = {};
-                for (int p = 0; p < pieces; p += 4) {
-                    float4 v[4][4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            v[i][j] = p + i < pieces && c0 + 8 * j < s.n ? __ldcg(reinterpret_cast<const float4*>(p0 + static_cast<size_t>(p + i) * (NT * 128) + (c0 + 8 * j) * 128))
-                                                                          : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) { sum[j].x += v[i][j].x; sum[j].y += v[i][j].y; sum[j].z += v[i][j].z; sum[j].w += v[i][j].w; }
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int m = c0 + 8 * j;
-                    if (m >= s.n) break;
-                    float* q = a.y + static_cast<size_t>(GROUPED ? __ldg(a.out_row + s.row0 + m) : s.row0 + m) * a.N + col4;
-                    if (vec) {
-                        if (col4 < a.N) *reinterpret_cast<float4*>(q) = sum[j];
-                    } else {
-                        const float e[4] = {sum[j].x, sum[j].y, sum[j].z, sum[j].w};
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (col4 + i < a.N) q[i] = e[i];
-                    }
-                }
+                __syncwarp();
             }
         }
     }
     __syncwarp();
     fence_before();
     __syncthreads();
+    if constexpr (CG == 2) {                       // neither CTA leaves while the other may still reach into it
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
     if (warp == 1) {
         fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
+        if constexpr (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
     }
 }
 
@@ -307,14 +380,24 @@ int launch_nt(const CUtensorMap& map, const MxArgs& a, cudaStream_t st) {
         if (rc) return rc;
         configured = true;
     }
+    constexpr int CG = Lay<NT>::CG;
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim = {CG, 1, 1};
+    cfg.gridDim = dim3(ctx().sm_count / CG * CG); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = Lay<NT>::BYTES; cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = CG == 2 ? 2 : 1;
     ctx().launches++;
-    return launch_early(mx_gemm_kernel<NT, GROUPED>, dim3(ctx().sm_count), THREADS, Lay<NT>::BYTES, st, map, a);
+    return cuda_check(cudaLaunchKernelEx(&cfg, mx_gemm_kernel<NT, GROUPED>, map, a), "mx_gemm launch");
 }
 
 }  // namespace
 
-// Partial sums: the c-th CTA's part of the t-th cut tile is number c + t.
-size_t mx_gemm_part_bytes(int nt, int cut_tiles) { return static_cast<size_t>(ctx().sm_count + cut_tiles) * nt * 128 * sizeof(float); }
+int mx_gemm_cg(int nt) { return cg_of(nt); }
+// Parts of cut tiles: two per CTA. Counters: two per cut tile and CTA of a pair, fewer than two tiles a unit.
+size_t mx_gemm_part_bytes(int nt) { return static_cast<size_t>(2 * ctx().sm_count) * nt * 128 * sizeof(float); }
+int    mx_gemm_counters() { return 4 * ctx().sm_count; }
 
 int launch_mx_gemm(const MxArgs& a, int nt, long long tiles, bool grouped, cudaStream_t st) {
     CUtensorMap map;

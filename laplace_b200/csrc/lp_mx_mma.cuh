@@ -9,26 +9,31 @@ namespace mx {
 
 #ifdef __CUDACC__
 
-// kind::mxf8f6f4: D fp32, A e2m1, B e4m3, both K-major, scales ue8m0; 128 rows of A, n of B; the byte of the scale words that this step takes
+// CG: CTAs that work on one product, 1 or 2 (a pair of SMs: 128 rows of A and half of B's in the shared memory of each).
+// kind::mxf8f6f4: D fp32, A e2m1, B e4m3, both K-major, scales ue8m0; 128 CG rows of A, n of B; the byte of the scale words that this step takes
+template <int CG>
 __device__ __forceinline__ uint32_t idesc_mx(int n, int byte) {
-    return (static_cast<uint32_t>(byte) << 4) | (5u << 7) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) | (8u << 24) | (static_cast<uint32_t>(byte) << 29);
+    return (static_cast<uint32_t>(byte) << 4) | (5u << 7) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) | (8u * CG << 24) | (static_cast<uint32_t>(byte) << 29);
 }
+template <int CG>
 __device__ __forceinline__ void mma_mx(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t acc) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-        :: "r"(d), "l"(ad), "l"(bd), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc) : "memory");
+    if constexpr (CG == 1)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+            :: "r"(d), "l"(ad), "l"(bd), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc) : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+            :: "r"(d), "l"(ad), "l"(bd), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc) : "memory");
 }
-// 32 rows of 16 bytes -> 4 TMEM columns of every quadrant; the first column a multiple of four
+// 32 rows of 16 bytes -> 4 TMEM columns of every quadrant (of both CTAs, each from its own shared memory); the first column a multiple of four
+template <int CG>
 __device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t smem) {
     const uint64_t d = static_cast<uint64_t>((smem >> 4) & 0x3fffu) | (static_cast<uint64_t>(128 >> 4) << 16) | (static_cast<uint64_t>(128 >> 4) << 32) | (static_cast<uint64_t>(1) << 46);
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" :: "r"(taddr), "l"(d) : "memory");
-}
-// Whether a barrier's phase is over, without waiting (try_wait may suspend the thread for a while).
-__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    return ok != 0;
+    if constexpr (CG == 1) asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" :: "r"(taddr), "l"(d) : "memory");
+    else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" :: "r"(taddr), "l"(d) : "memory");
 }
 // 32 lanes x 8 columns
 __device__ __forceinline__ void ld8(uint32_t taddr, float (&v)[8]) {

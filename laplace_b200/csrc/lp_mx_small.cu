@@ -148,11 +148,11 @@ __global__ void __launch_bounds__(THREADS, 2) mx_small_kernel(const __grid_const
                 fence_after();
                 const uint32_t sfa = tmem + SF_COL + 8 * set, sfb = sfa + 4;
                 set ^= 1;
-                copy_scales(sfa, sb + off_sfa + st * SF_TILE);
-                copy_scales(sfb, sb + off_sfb + st * SF_TILE);
+                copy_scales<1>(sfa, sb + off_sfa + st * SF_TILE);
+                copy_scales<1>(sfb, sb + off_sfb + st * SF_TILE);
                 const uint64_t ad = smem_desc_sw128(sb + st * A_STAGE), bd = smem_desc_sw128(sb + off_b + st * B_STAGE);
 #pragma unroll
-                for (int ks = 0; ks < 4; ++ks) mma_mx(tmem + acc * N_MMA, ad + 2 * ks, bd + 2 * ks, idesc_mx(N_MMA, ks), sfa, sfb, kt != k0 || ks);
+                for (int ks = 0; ks < 4; ++ks) mma_mx<1>(tmem + acc * N_MMA, ad + 2 * ks, bd + 2 * ks, idesc_mx<1>(N_MMA, ks), sfa, sfb, kt != k0 || ks);
                 commit(bar(f.empty[st]));
                 if (++st == S) { st = 0; parity ^= 1; }
             }
