@@ -18,6 +18,7 @@
 #include <cuda_bf16.h>
 
 #include "lp_mx.cuh"
+#include "lp_mx_mma.cuh"
 
 namespace lp {
 namespace {
@@ -189,7 +190,7 @@ __device__ __forceinline__ int pair_expert_of(const int* pair_expert, const int*
     return p >= P || e < 0 ? -1 : bad ? -2 : e;
 }
 __global__ void __launch_bounds__(1024) mx_group_kernel(const int* __restrict__ pair_expert, const int* __restrict__ pair_row, int P, int E, int x_rows, int tile_w, int tile_groups,
-                                                        int2* __restrict__ place, int* __restrict__ out_row, int4* __restrict__ tab, int4* __restrict__ work, int row_tiles, int nt, int kts, int n, int* err) {
+                                                        int2* __restrict__ place, int* __restrict__ out_row, int4* __restrict__ tab, int4* __restrict__ work, int row_tiles, int kts, int n, int* err) {
     extern __shared__ int sm[];
     const int W = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int* start = sm;                       // first row of an expert in the image
@@ -243,8 +244,8 @@ __global__ void __launch_bounds__(1024) mx_group_kernel(const int* __restrict__ 
         }
         // how the tiles are shared out (cut_of): a number of parts per lane
         const int all = tiles * row_tiles, most = most_parts(all, kts, n);
-        const int best = __reduce_min_sync(0xffffffffu, lane < most ? cut_cost(nt, kts, lane + 1) * MAX_PARTS + lane : 0x7fffffff);
-        const Cut c = cut_of(nt, all, kts, n, best % MAX_PARTS + 1, best / MAX_PARTS);
+        const int best = __reduce_min_sync(0xffffffffu, lane < most ? cut_cost(kts, lane + 1) * MAX_PARTS + lane : 0x7fffffff);
+        const Cut c = cut_of(all, kts, n, best % MAX_PARTS + 1, best / MAX_PARTS);
         if (lane == 0) *work = make_int4(c.tiles, c.cut, c.ctas, 0);
     }
     __syncthreads();
@@ -294,10 +295,10 @@ Plan plan_of(int rows, int experts, int K, int N) {
     const int per = experts ? (rows + experts - 1) / experts : rows;
     p.nt = per <= 32 ? 32 : per <= 64 ? 64 : per <= 128 ? 128 : 256;
     p.tiles_m = (rows + p.nt - 1) / p.nt;
-    const int cg = mx_gemm_cg(p.nt);
-    p.row_tiles = (p.rts + cg - 1) / cg;
+    const bool pairs = p.nt == 256;
+    p.row_tiles = pairs ? (p.rts + 1) / 2 : p.rts;
     p.tile_w = experts ? p.nt : ((rows + p.tiles_m - 1) / p.tiles_m + 31) & ~31;
-    p.n_counters = mx_gemm_counters();
+    p.n_counters = pairs ? mx_pair_counters() : 0;
     p.tile_groups = (p.nt + 127) / 128;
     p.max_tiles = experts ? rows / p.tile_w + (experts < rows ? experts : rows) : p.tiles_m;
     p.groups = p.max_tiles * p.tile_groups;
@@ -306,7 +307,7 @@ Plan plan_of(int rows, int experts, int K, int N) {
     p.img = take(static_cast<size_t>(p.kts) * p.img_rows * 128);
     p.sf = take(static_cast<size_t>(p.kts) * p.groups * SF_TILE);
     p.counters = take(p.n_counters * sizeof(unsigned));
-    p.part = take(mx_gemm_part_bytes(p.nt));
+    p.part = take(pairs ? mx_pair_part_bytes() : 0);
     if (experts) {
         p.place = take(static_cast<size_t>(rows) * sizeof(int2));
         p.out_row = take(static_cast<size_t>(p.img_rows) * 4);
@@ -330,7 +331,7 @@ int launch_product(const float* x, int x_rows, const uint8_t* packed, const int*
     a.M = rows; a.N = N; a.kts = p.kts; a.rts = p.rts; a.img_rows = p.img_rows; a.groups = p.groups; a.tile_w = p.tile_w; a.tiles_m = p.tiles_m; a.tile_groups = p.tile_groups; a.row_tiles = p.row_tiles;
     a.part = reinterpret_cast<float*>(ws + p.part); a.counters = reinterpret_cast<unsigned*>(ws + p.counters); a.err = c.d_err;
     int2* place = nullptr;
-    const int units = c.sm_count / mx_gemm_cg(p.nt);
+    const int units = c.sm_count / 2;
     int rc;
     if (GROUPED) {
         place = reinterpret_cast<int2*>(ws + p.place);
@@ -344,23 +345,29 @@ int launch_product(const float* x, int x_rows, const uint8_t* packed, const int*
             configured = true;
         }
         rc = launch_early(mx_group_kernel, dim3(1), warps * 32, (warps + 2) * static_cast<size_t>(experts) * sizeof(int), st, pair_expert, pair_row, rows, experts, x_rows, p.tile_w,
-                          p.tile_groups, place, reinterpret_cast<int*>(ws + p.out_row), reinterpret_cast<int4*>(ws + p.tab), reinterpret_cast<int4*>(ws + p.work), p.row_tiles, p.nt, p.kts, units, c.d_err);
+                          p.tile_groups, place, reinterpret_cast<int*>(ws + p.out_row), reinterpret_cast<int4*>(ws + p.tab), reinterpret_cast<int4*>(ws + p.work), p.row_tiles, p.kts, units, c.d_err);
         c.launches++;
         if (rc) return rc;
     }
     if (!GROUPED) {
-        const int tiles = p.tiles_m * p.row_tiles, most = most_parts(tiles, p.kts, units);
-        int parts = 1;
-        for (int q = 2; q <= most; ++q)
-            if (cut_cost(p.nt, p.kts, q) < cut_cost(p.nt, p.kts, parts)) parts = q;
-        a.dense = cut_of(p.nt, tiles, p.kts, units, parts, cut_cost(p.nt, p.kts, parts));
+        a.dense = Cut{p.tiles_m * p.row_tiles, 0, 0};
+        if (p.nt == 256) {
+            const int most = most_parts(a.dense.tiles, p.kts, units);
+            int parts = 1;
+            for (int q = 2; q <= most; ++q)
+                if (cut_cost(p.kts, q) < cut_cost(p.kts, parts)) parts = q;
+            a.dense = cut_of(a.dense.tiles, p.kts, units, parts, cut_cost(p.kts, parts));
+        }
     }
     const long long warps = static_cast<long long>(rows) * ((p.kts + 1) / 2);
     rc = launch_early(mx_act_kernel<GROUPED>, dim3(static_cast<unsigned>((warps + 7) / 8)), 256, 0, st, x, K, p.kts, rows, ActDst{ws + p.img, ws + p.sf, p.img_rows, p.groups, p.tile_w, p.tile_groups},
                       pair_row, static_cast<const int2*>(place), reinterpret_cast<unsigned*>(ws + p.counters), p.n_counters);
     c.launches++;
     if (rc) return rc;
-    return launch_mx_gemm(a, p.nt, static_cast<long long>(GROUPED ? experts : 1) * p.rts * p.kts, GROUPED, st);
+    CUtensorMap map;
+    if (!mx_weights_map(&map, a.q, static_cast<size_t>(GROUPED ? experts : 1) * p.rts * p.kts)) return LAPLACE_ERR_CUDA;
+    if (p.nt == 256) return launch_mx_pair(map, a, GROUPED, st);
+    return launch_mx_mid(map, a, p.nt, static_cast<long long>(GROUPED ? (experts < rows ? experts : rows) : 1) * p.rts, GROUPED, st);
 }
 
 // rows: token tiles times row tiles are counted in 32 bits

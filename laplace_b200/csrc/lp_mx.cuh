@@ -1,6 +1,7 @@
 // lp_mx.cuh - what the MXFP4 kernels share: sizes of the packed layout (lp_mx.cu), conversions, arguments of a product.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 
 #include "lp_common.cuh"
@@ -15,21 +16,20 @@ constexpr int SF_TILE = 512;          // bytes of their scales: 128 rows x 4
 // begin with a group of their own (the tensor core takes them from TMEM columns whose number is a multiple of four).
 struct ActDst { uint8_t* img; uint8_t* sf; int rows, groups, tile_w, tile_groups; };
 
-// Tiles of 128 (pairs: 256) weight rows by up to NT tokens, over n CTAs (pairs of them). `cut` of `tiles` are cut, over `ctas` of these.
+// Tiles of 256 weight rows x 256 tokens over n pairs of SMs: `cut` of `tiles` are cut, over `ctas` pairs.
 struct Cut { int tiles, cut, ctas; };
-// What a cut costs, in k steps of a whole tile: CUT_COST once, and for every part of a tile that is read back (NT x 512 bytes) its own.
-constexpr int CUT_COST = 5;
-__host__ __device__ inline int piece_cost(int nt) { return nt == 256 ? 5 : nt == 128 ? 3 : nt == 64 ? 2 : 1; }
-__host__ __device__ inline int cut_cost(int nt, int kts, int parts) { return parts == 1 ? kts : (kts + parts - 1) / parts + CUT_COST + (parts - 1) * piece_cost(nt); }
+// What a cut costs, in k steps of a whole tile (512 cycles): once, and for every part of a tile that is read back (128 KB a CTA).
+constexpr int CUT_COST = 14, PIECE_COST = 6;
+__host__ __device__ inline int cut_cost(int kts, int parts) { return parts == 1 ? kts : (kts + parts - 1) / parts + CUT_COST + (parts - 1) * PIECE_COST; }
 constexpr int MAX_PARTS = 32;
-// The tiles behind the last whole round are a round of their own, or each of them is cut in as many parts as cost least (best, their cost),
-// or they and the last whole round are cut over all n.
-__host__ __device__ inline Cut cut_of(int nt, int tiles, int kts, int n, int parts, int cost) {
+// The tiles behind the last whole round are a round of their own, or each of them is cut in `parts` parts (the number that costs least, and
+// its cost), or they and the last whole round are cut over all n.
+__host__ __device__ inline Cut cut_of(int tiles, int kts, int n, int parts, int cost) {
     Cut c{tiles, 0, 0};
     const int left = tiles % n;
     if (!left) return c;
     if (parts > 1) { c.cut = left; c.ctas = left * parts; }
-    if (tiles > n && static_cast<int>((static_cast<long long>(left) * kts + n - 1) / n) + CUT_COST + piece_cost(nt) < cost) { c.cut = left + n; c.ctas = n; }
+    if (tiles > n && static_cast<int>((static_cast<long long>(left) * kts + n - 1) / n) + CUT_COST + PIECE_COST < cost) { c.cut = left + n; c.ctas = n; }
     return c;
 }
 __host__ __device__ inline int most_parts(int tiles, int kts, int n) {
@@ -50,7 +50,7 @@ struct MxArgs {
     const int4*    work;         // {row tiles of all token tiles, how many of them are cut, over how many units, -}
     const int*     out_row;
     int            tiles_m;      // token tiles of one matrix
-    int            row_tiles;    // row tiles of a matrix: rts, or of pairs of CTAs
+    int            row_tiles;    // row tiles of a matrix: rts, or those of 256 rows
     float*         part;         // parts of cut tiles, and their counters
     unsigned*      counters;
     int*           err;
@@ -130,11 +130,11 @@ __device__ __forceinline__ uint2 mxfp8_block8(const float (&v)[8], int lane, uin
 
 }  // namespace mx
 
-int    mx_gemm_cg(int nt);
-size_t mx_gemm_part_bytes(int nt);
-int    mx_gemm_counters();
+size_t mx_pair_part_bytes();
+int    mx_pair_counters();
+int    launch_mx_pair(const CUtensorMap& map, const mx::MxArgs& a, bool grouped, cudaStream_t st);
+int    launch_mx_mid(const CUtensorMap& map, const mx::MxArgs& a, int nt, long long tiles, bool grouped, cudaStream_t st);
 bool   mx_small_takes(int rows, bool grouped);
 int    launch_mx_small(const float* x, int x_rows, const uint8_t* packed, const int* pair_expert, const int* pair_row, int rows, int experts, float* y, int K, int N, cudaStream_t st);
-int    launch_mx_gemm(const mx::MxArgs& a, int nt, long long tiles, bool grouped, cudaStream_t st);
 
 }  // namespace lp

@@ -1,18 +1,16 @@
-// lp_mx_gemm.cu - products of packed MXFP4 weights and MXFP8 activations on the block-scaled tensor core instruction
-// (tcgen05.mma kind::mxf8f6f4): D[128 weight rows][up to NT tokens] += A * B, 32 values a step, both scaled by a power of two per 32 values.
-// Formats and layouts: lp_mx.cu. The instruction takes the 4-bit weights and their scale bytes as they lie in memory: no thread
-// touches a weight. TMA spreads the 8 bytes of 16 values over 16 bytes of shared memory on the way in, the form that the instruction reads.
+// lp_mx_pair.cu - products of packed MXFP4 weights and quantized rows on pairs of SMs (cta_group::2), tiles of 256 weight rows x up to 256 tokens: more
+// than 128 rows of one matrix, or experts with more than 128 pairs on average. Formats and layouts: lp_mx.cu, the instruction: lp_mx_mma.cuh.
 //
-// Work. Tiles of 128 weight rows x NT tokens, k in steps of 128, G CTAs (one per SM). Whole tiles go to the CTAs one after the other; the last ones, where
-// they do not come out even, may be cut: their k steps, in tile order, go in equal runs to the CTAs (cut_of in lp_mx.cuh says when that pays). Of a
-// cut tile's CTAs the last one to arrive (a counter) keeps its sums in registers; the others leave theirs in the workspace, on which
+// Either CTA of a pair has its 128 weight rows and half of the tokens in shared memory. What bounds one CTA with 128 x 256 is the way from L2, 41 KB a
+// k step of 128 that takes the tensor core 512 cycles; a pair's CTAs take 25 KB each.
+//
+// Work. Tiles over G pairs, whole ones one after the other; the last ones, where they do not come out even, may be cut: their k steps, in tile
+// order, go in equal runs to the pairs (cut_of in lp_mx.cuh says when that pays). Of a
+// cut tile's pairs the last one to arrive (a counter) keeps its sums in registers; the others leave theirs in the workspace, on which
 // it waits - they are running, so it does not wait long - and it adds all up in the order of k: the result does not depend on who was last.
 //
-// More than 128 tokens a tile: a pair of SMs (cta_group::2) takes 256 weight rows x 256 tokens, each CTA with its 128 rows and half of the tokens
-// in shared memory. What bounds one CTA with 128 x 256 is the way from L2: 41 KB a step of 512 cycles; a pair's CTAs take 25 KB each.
-//
-// Roles by warp: 0 copies, 1 MMA issue (owns the TMEM), 4-11 drain (lane = weight row). All waits are bounded; a wait that gives up
-// raises the status word and the roles leave their loops.
+// Roles by warp: 0 copies, 1 MMA issue in the even CTA (owns the TMEM), word of the filled stages in the odd one, 4-11 drain (lane =
+// weight row). All waits are bounded; a wait that gives up raises the status word and the roles leave their loops.
 #include "lp_mx.cuh"
 #include "lp_mx_mma.cuh"
 #include "lp_tc.cuh"
@@ -28,23 +26,19 @@ constexpr int DRAIN = 256;                     // threads of the drain: two warp
 constexpr int A_STAGE = 128 * 128;             // 128 rows x 128 values, a byte each after the copy
 constexpr uint32_t SF_COL = 480;               // TMEM columns of the scales: two sets of 16 (4 of the weights, up to 8 of the activations)
 
-// CTAs of a tile of NT tokens.
-constexpr int cg_of(int nt) { return nt == 256 ? 2 : 1; }
-
-template <int NT> struct Lay {
-    static constexpr int CG = cg_of(NT), B_STAGE = NT / CG * 128;
+constexpr int NT = 256;                        // tokens of a tile
+struct Lay {
+    static constexpr int B_STAGE = NT / 2 * 128;
     static constexpr int GROUPS = (NT + 127) / 128;       // 128-row groups of scales
     static constexpr int STAGE = A_STAGE + B_STAGE + SF_TILE + GROUPS * SF_TILE;
     static constexpr int STAGES = (226 * 1024 - 1024) / STAGE;
-    static constexpr int ACCS = NT == 256 ? 1 : 2;
     static constexpr uint32_t A = 0, B = A + STAGES * A_STAGE, SFA = B + STAGES * B_STAGE, SFB = SFA + STAGES * SF_TILE, BAR = SFB + STAGES * GROUPS * SF_TILE;
     static constexpr uint32_t FULL = BAR, EMPTY = FULL + 8 * STAGES, TFULL = EMPTY + 8 * STAGES, TEMPTY = TFULL + 16, PTR = TEMPTY + 16, ABORT = PTR + 4, SAY = ABORT + 4,
                               BYTES = SAY + 8 + 1024;
     static_assert(BYTES <= 227 * 1024, "shared memory");
-    static_assert(ACCS * NT <= SF_COL, "TMEM columns");
 };
 
-// rt: row tile, of 128 or (pairs) 256 rows
+// rt: row tile, of 256 rows
 struct Seg { int expert, rt, row0, n, group, k0, k1, cut; };      // group: first 128-row group of its scales; cut: number of the cut tile, -1 for a whole one
 struct Work { int tiles, cut, ctas; long long units; };
 
@@ -74,14 +68,14 @@ __device__ __forceinline__ void tile_at(const MxArgs& a, int t, Seg& s) {
     }
 }
 // A unit's work piece by piece, in the order in which every role walks it.
-template <bool GROUPED, int CG>
+template <bool GROUPED>
 struct Walk {
     const MxArgs& a;
     const Work w;
     long long u, u1;
     int next;
     __device__ __forceinline__ Walk(const MxArgs& args, const Work& work) : a(args), w(work) {
-        const int c = blockIdx.x / CG;
+        const int c = blockIdx.x / 2;
         u = c < w.ctas ? cut_start(w, c) : 0;
         u1 = c < w.ctas ? cut_start(w, c + 1) : 0;
         next = w.cut + c;
@@ -100,7 +94,7 @@ struct Walk {
         if (next >= w.tiles) return false;
         tile_at<GROUPED>(a, next, s);
         s.k0 = 0; s.k1 = a.kts; s.cut = -1;
-        next += gridDim.x / CG;
+        next += gridDim.x / 2;
         return true;
     }
 };
@@ -114,37 +108,30 @@ __device__ __forceinline__ bool any_of(int bar, bool mine) {
     return r != 0;
 }
 
-template <int NT, bool GROUPED>
-__global__ void __launch_bounds__(THREADS, 1) mx_gemm_kernel(const __grid_constant__ CUtensorMap map, const MxArgs a) {
-    using L = Lay<NT>;
-    constexpr int CG = L::CG;
+template <bool GROUPED>
+__global__ void __launch_bounds__(THREADS, 1) mx_pair_kernel(const __grid_constant__ CUtensorMap map, const MxArgs a) {
+    using L = Lay;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t sb = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem = smem_raw + (sb - smem_u32(smem_raw));
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::ABORT);
-    const int warp = threadIdx.x >> 5, rank = CG == 2 ? static_cast<int>(pair_rank()) : 0;
+    const int warp = threadIdx.x >> 5, rank = static_cast<int>(pair_rank());
     if (threadIdx.x == 0) {
-        for (int i = 0; i < L::STAGES; ++i) { mbar_init(sb + L::FULL + 8 * i, CG - rank); mbar_init(sb + L::EMPTY + 8 * i, 1); }      // the even CTA's: its own copies and word of the other's
-        for (int i = 0; i < 2; ++i) { mbar_init(sb + L::TFULL + 8 * i, 1); mbar_init(sb + L::TEMPTY + 8 * i, CG * DRAIN / 32); }
+        for (int i = 0; i < L::STAGES; ++i) { mbar_init(sb + L::FULL + 8 * i, 2 - rank); mbar_init(sb + L::EMPTY + 8 * i, 1); }      // the even CTA's: its own copies and word of the other's
+        mbar_init(sb + L::TFULL, 1);
+        mbar_init(sb + L::TEMPTY, 2 * DRAIN / 32);
         *abort_flag = 0;
         fence_barrier_init();
         asm volatile("prefetch.tensormap [%0];" :: "l"(&map) : "memory");
     }
     if (warp == 1) {
-        if constexpr (CG == 2) {
-            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(sb + L::PTR), "r"(512u) : "memory");
-            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-        } else {
-            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(sb + L::PTR), "r"(512u) : "memory");
-            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-        }
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(sb + L::PTR), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     fence_before();
     __syncthreads();
-    if constexpr (CG == 2) {                       // both CTAs' barriers are there before either arrives on them
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    }
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");        // both CTAs' barriers are there before either arrives on them
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + L::PTR);
     // Experts: the table of token tiles is made by the kernels before this one. One matrix: the weights may be copied meanwhile; the quantizer
@@ -154,13 +141,12 @@ __global__ void __launch_bounds__(THREADS, 1) mx_gemm_kernel(const __grid_consta
     const Work w{cut.x, cut.y, cut.z, static_cast<long long>(cut.y) * a.kts};
 
     if (warp < 4) {
-    if constexpr (NT == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");       // 128 x 64 + 256 x 216 of 384 x 168 registers
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");       // 128 x 64 + 256 x 216 of 384 x 168 registers
     if (warp == 0 && elect_one()) {
         // of this CTA: its row tile (of an odd number the last one twice, the second time for nothing), its part of the tokens
-        auto tile_of = [&](const Seg& s, int kt) { return (static_cast<size_t>(s.expert) * a.rts + min(s.rt * CG + rank, a.rts - 1)) * a.kts + kt; };
+        auto tile_of = [&](const Seg& s, int kt) { return (static_cast<size_t>(s.expert) * a.rts + min(s.rt * 2 + rank, a.rts - 1)) * a.kts + kt; };
         auto rows_of = [&](const Seg& s, int& first) {
             const int n8 = (s.n + 7) & ~7, half = ((s.n + 31) & ~31) / 2;
-            if (CG == 1) { first = 0; return n8; }
             first = rank * half;
             return rank ? max(n8 - half, 0) : min(n8, half);
         };
@@ -182,13 +168,13 @@ __global__ void __launch_bounds__(THREADS, 1) mx_gemm_kernel(const __grid_consta
         };
         int early = 0;
         if (!GROUPED) {
-            Walk<GROUPED, CG> walk(a, w);
+            Walk<GROUPED> walk(a, w);
             Seg s;
             while (early < L::STAGES && walk(s))
                 for (int kt = s.k0; kt < s.k1 && early < L::STAGES; ++kt) weights(early++, s, kt);
             asm volatile("griddepcontrol.wait;" ::: "memory");
         }
-        Walk<GROUPED, CG> walk(a, w);
+        Walk<GROUPED> walk(a, w);
         Seg s;
         int it = 0;
         bool ok = true;
@@ -202,41 +188,33 @@ __global__ void __launch_bounds__(THREADS, 1) mx_gemm_kernel(const __grid_consta
         if (!ok)                                        // what is in flight lands before the CTA goes
             for (int i = 0; i < 1000; ++i) __nanosleep(1000);
     } else if (warp == 1 && rank == 0 && elect_one()) {
-        Walk<GROUPED, CG> walk(a, w);
+        Walk<GROUPED> walk(a, w);
         Seg s;
         int it = 0;
         bool ok = true;
-        auto wait = [&](uint32_t bar, int parity, int code) {
-            return CG == 2 ? wait_pair(bar, parity, abort_flag, a.err, code) : wait_or_abort<true>(bar, parity, abort_flag, a.err, code);
-        };
-        auto done = [&](uint32_t bar) {
-            if constexpr (CG == 2) commit_pair(bar);
-            else commit(bar);
-        };
         for (int seg = 0; ok && walk(s); ++seg) {
-            const int acc = seg % L::ACCS, n = CG == 2 ? (s.n + 31) & ~31 : (s.n + 15) & ~15, groups = (s.n + 127) >> 7;
-            const uint32_t d = tmem + acc * NT;
-            if (seg >= L::ACCS && !wait(sb + L::TEMPTY + 8 * acc, (seg / L::ACCS - 1) & 1, DEV_TIMEOUT_TMEM)) { ok = false; break; }
+            const int n = (s.n + 31) & ~31, groups = (s.n + 127) >> 7;
+            if (seg && !wait_pair(sb + L::TEMPTY, (seg - 1) & 1, abort_flag, a.err, DEV_TIMEOUT_TMEM)) { ok = false; break; }
             fence_after();
             for (int kt = s.k0; kt < s.k1; ++kt, ++it) {
                 const int st = it % L::STAGES;
-                if (!wait(sb + L::FULL + 8 * st, (it / L::STAGES) & 1, DEV_TIMEOUT_FULL)) { ok = false; break; }
+                if (!wait_pair(sb + L::FULL + 8 * st, (it / L::STAGES) & 1, abort_flag, a.err, DEV_TIMEOUT_FULL)) { ok = false; break; }
                 fence_after();
                 const uint32_t sfa = tmem + SF_COL + 16 * (it & 1), sfb = sfa + 4;
-                copy_scales<CG>(sfa, sb + L::SFA + st * SF_TILE);
-                for (int g = 0; g < groups; ++g) copy_scales<CG>(sfb + 4 * g, sb + L::SFB + (st * L::GROUPS + g) * SF_TILE);
+                copy_scales<2>(sfa, sb + L::SFA + st * SF_TILE);
+                for (int g = 0; g < groups; ++g) copy_scales<2>(sfb + 4 * g, sb + L::SFB + (st * L::GROUPS + g) * SF_TILE);
                 const uint64_t ad = smem_desc_sw128(sb + L::A + st * A_STAGE), bd = smem_desc_sw128(sb + L::B + st * L::B_STAGE);
 #pragma unroll
-                for (int ks = 0; ks < 4; ++ks) mma_mx<CG>(d, ad + 2 * ks, bd + 2 * ks, idesc_mx<CG>(n, ks), sfa, sfb, kt != s.k0 || ks);
-                done(sb + L::EMPTY + 8 * st);
+                for (int ks = 0; ks < 4; ++ks) mma_mx<2>(tmem, ad + 2 * ks, bd + 2 * ks, idesc_mx<2>(n, ks), sfa, sfb, kt != s.k0 || ks);
+                commit_pair(sb + L::EMPTY + 8 * st);
             }
-            if (ok) done(sb + L::TFULL + 8 * acc);
+            if (ok) commit_pair(sb + L::TFULL);
         }
         if (!ok)                                        // what has been issued ends before the CTA goes
             for (int i = 0; i < 1000; ++i) __nanosleep(1000);
-    } else if (CG == 2 && warp == 1 && rank == 1 && elect_one()) {      // (elect takes the whole warp: no lane of the even CTA's may come here)
+    } else if (warp == 1 && rank == 1 && elect_one()) {      // (elect takes the whole warp: no lane of the even CTA's may come here)
         // the odd CTA: tells the even one of its stages as they fill
-        Walk<GROUPED, CG> walk(a, w);
+        Walk<GROUPED> walk(a, w);
         Seg s;
         int it = 0;
         bool ok = true;
@@ -248,39 +226,38 @@ __global__ void __launch_bounds__(THREADS, 1) mx_gemm_kernel(const __grid_consta
             }
     }
     } else {
-        if constexpr (NT == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-        Walk<GROUPED, CG> walk(a, w);
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        Walk<GROUPED> walk(a, w);
         Seg s;
         const int lane = threadIdx.x & 31, id = threadIdx.x - 128, half = id >> 7, r = id & 127;      // r: weight row of the tile
         const uint32_t quadrant = static_cast<uint32_t>(warp & 3) * 32u << 16;
         volatile int* say = reinterpret_cast<volatile int*>(smem + L::SAY);
         for (int seg = 0; walk(s); ++seg) {
-            const int acc = seg % L::ACCS;
-            const bool ok = wait_or_abort<false>(sb + L::TFULL + 8 * acc, (seg / L::ACCS) & 1, abort_flag, a.err, DEV_TIMEOUT_MMA);
+            const bool ok = wait_or_abort<false>(sb + L::TFULL, seg & 1, abort_flag, a.err, DEV_TIMEOUT_MMA);
             // the warps meet at cut tiles (which come first): they leave together or not at all
             if (s.cut >= 0 ? any_of<DRAIN>(1, !ok) : !ok) break;
             __syncwarp();
             fence_after();
-            const int rt = s.rt * CG + rank, col = rt * 128 + r, unit = blockIdx.x / CG;
+            const int rt = s.rt * 2 + rank, col = rt * 128 + r, unit = blockIdx.x / 2;
             // Columns 32 half + 64 j .. + 31: all into registers first, so that the next tile's products do not wait for what follows.
-            constexpr int J = NT < 64 ? 1 : NT / 64;
+            constexpr int J = NT / 64;
             float v[J][32];
 #pragma unroll
             for (int j = 0; j < J; ++j)
-                if (32 * half + 64 * j < s.n) ld32(tmem + quadrant + acc * NT + 32 * half + 64 * j, v[j]);
+                if (32 * half + 64 * j < s.n) ld32(tmem + quadrant + 32 * half + 64 * j, v[j]);
             wait_ld();
             fence_before();
             __syncwarp();
             if (lane == 0) {
-                if (rank == 0) mbar_arrive(sb + L::TEMPTY + 8 * acc);
-                else arrive_cluster(map_to_rank(sb + L::TEMPTY + 8 * acc, 0));
+                if (rank == 0) mbar_arrive(sb + L::TEMPTY);
+                else arrive_cluster(map_to_rank(sb + L::TEMPTY, 0));
             }
             const int full = half ? max(0, s.n - 32) : s.n;      // (columns of the tile from this half's first on)
             if (s.cut >= 0) {
                 const long long u = static_cast<long long>(s.cut) * a.kts;
                 const int first = cut_owner(w, u), pieces = cut_owner(w, u + a.kts - 1) - first + 1;
-                unsigned* count = a.counters + 2 * (s.cut * CG + rank);      // {arrived, written}
-                auto part = [&](int c, bool begins) { return a.part + static_cast<size_t>(slot_of(c, begins) * CG + rank) * (NT * 128) + half * (32 * 128) + r; };
+                unsigned* count = a.counters + 2 * (s.cut * 2 + rank);      // {arrived, written}
+                auto part = [&](int c, bool begins) { return a.part + static_cast<size_t>(slot_of(c, begins) * 2 + rank) * (NT * 128) + (half * (8 * 128) + r) * 4; };      // [column / 4][row][4 columns]
                 if (id == 0) *say = atomicAdd(count, 1u) == static_cast<unsigned>(pieces - 1);
                 named_bar_sync(1, DRAIN);
                 const bool last = *say;
@@ -289,8 +266,8 @@ __global__ void __launch_bounds__(THREADS, 1) mx_gemm_kernel(const __grid_consta
 #pragma unroll
                     for (int j = 0; j < J; ++j)
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (64 * j + i < full) __stcg(q + (64 * j + i) * 128, v[j][i]);
+                        for (int i = 0; i < 32; i += 4)
+                            if (64 * j + i < full) __stcg(reinterpret_cast<float4*>(q + (64 * j + i) * 128), make_float4(v[j][i], v[j][i + 1], v[j][i + 2], v[j][i + 3]));
                     named_bar_sync(1, DRAIN);
                     if (id == 0) { __threadfence(); atomicAdd(count + 1, 1u); }
                     continue;
@@ -307,28 +284,27 @@ __global__ void __launch_bounds__(THREADS, 1) mx_gemm_kernel(const __grid_consta
                 }
                 if (any_of<DRAIN>(1, !there)) break;
 #pragma unroll
-                for (int b = 0; b < 2 * J; ++b) {            // sixteen columns at a time
-                    const int c0 = 64 * (b / 2) + 16 * (b % 2);
-                    if (c0 >= full) break;
-                    float sum[16];
+                for (int j = 0; j < J; ++j) {
+                    if (64 * j >= full) break;
+                    float sum[32];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) sum[i] = 0.f;
+                    for (int i = 0; i < 32; ++i) sum[i] = 0.f;
 #pragma unroll 1
                     for (int p = 0; p < pieces; ++p) {
                         if (first + p == unit) {
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) sum[i] += v[b / 2][16 * (b % 2) + i];
+                            for (int i = 0; i < 32; ++i) sum[i] += v[j][i];
                         } else {
-                            const float* q = part(first + p, p == 0) + c0 * 128;
-                            float o[16];
+                            const float* q = part(first + p, p == 0) + j * (64 * 128);
+                            float4 o[8];
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) o[i] = c0 + i < full ? __ldcg(q + i * 128) : 0.f;
+                            for (int i = 0; i < 8; ++i) o[i] = 64 * j + 4 * i < full ? __ldcg(reinterpret_cast<const float4*>(q + i * 512)) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) sum[i] += o[i];
+                            for (int i = 0; i < 8; ++i) { sum[4 * i] += o[i].x; sum[4 * i + 1] += o[i].y; sum[4 * i + 2] += o[i].z; sum[4 * i + 3] += o[i].w; }
                         }
                     }
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) v[b / 2][16 * (b % 2) + i] = sum[i];
+                    for (int i = 0; i < 32; ++i) v[j][i] = sum[i];
                 }
             }
 #pragma unroll
@@ -361,59 +337,39 @@ __global__ void __launch_bounds__(THREADS, 1) mx_gemm_kernel(const __grid_consta
     __syncwarp();
     fence_before();
     __syncthreads();
-    if constexpr (CG == 2) {                       // neither CTA leaves while the other may still reach into it
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    }
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");        // neither CTA leaves while the other may still reach into it
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (warp == 1) {
         fence_after();
-        if constexpr (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
-        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
     }
 }
 
-template <int NT, bool GROUPED>
-int launch_nt(const CUtensorMap& map, const MxArgs& a, cudaStream_t st) {
+template <bool GROUPED>
+int launch(const CUtensorMap& map, const MxArgs& a, cudaStream_t st) {
     static bool configured = false;
     if (!configured) {
-        const int rc = cuda_check(cudaFuncSetAttribute(mx_gemm_kernel<NT, GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<NT>::BYTES), "mx_gemm shared memory");
+        const int rc = cuda_check(cudaFuncSetAttribute(mx_pair_kernel<GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay::BYTES), "mx_pair shared memory");
         if (rc) return rc;
         configured = true;
     }
-    constexpr int CG = Lay<NT>::CG;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim = {CG, 1, 1};
-    cfg.gridDim = dim3(ctx().sm_count / CG * CG); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = Lay<NT>::BYTES; cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = CG == 2 ? 2 : 1;
+    attr[1].val.clusterDim.x = 2; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(ctx().sm_count / 2 * 2); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = Lay::BYTES; cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = 2;
     ctx().launches++;
-    return cuda_check(cudaLaunchKernelEx(&cfg, mx_gemm_kernel<NT, GROUPED>, map, a), "mx_gemm launch");
+    return cuda_check(cudaLaunchKernelEx(&cfg, mx_pair_kernel<GROUPED>, map, a), "mx_pair launch");
 }
 
 }  // namespace
 
-int mx_gemm_cg(int nt) { return cg_of(nt); }
-// Parts of cut tiles: two per CTA. Counters: two per cut tile and CTA of a pair, fewer than two tiles a unit.
-size_t mx_gemm_part_bytes(int nt) { return static_cast<size_t>(2 * ctx().sm_count) * nt * 128 * sizeof(float); }
-int    mx_gemm_counters() { return 4 * ctx().sm_count; }
+// Parts of cut tiles: two per CTA. Counters: two per cut tile and CTA of a pair, fewer than two tiles a pair.
+size_t mx_pair_part_bytes() { return static_cast<size_t>(2 * ctx().sm_count) * NT * 128 * sizeof(float); }
+int    mx_pair_counters() { return 4 * ctx().sm_count; }
 
-int launch_mx_gemm(const MxArgs& a, int nt, long long tiles, bool grouped, cudaStream_t st) {
-    CUtensorMap map;
-    if (!mx_weights_map(&map, a.q, static_cast<size_t>(tiles))) return LAPLACE_ERR_CUDA;
-    if (grouped) switch (nt) {
-        case 32: return launch_nt<32, true>(map, a, st);
-        case 64: return launch_nt<64, true>(map, a, st);
-        case 128: return launch_nt<128, true>(map, a, st);
-        default: return launch_nt<256, true>(map, a, st);
-    }
-    switch (nt) {
-        case 32: return launch_nt<32, false>(map, a, st);
-        case 64: return launch_nt<64, false>(map, a, st);
-        case 128: return launch_nt<128, false>(map, a, st);
-        default: return launch_nt<256, false>(map, a, st);
-    }
-}
+int launch_mx_pair(const CUtensorMap& map, const MxArgs& a, bool grouped, cudaStream_t st) { return grouped ? launch<true>(map, a, st) : launch<false>(map, a, st); }
 
 }  // namespace lp

@@ -1,5 +1,5 @@
 // lp_mx_small.cu - products of packed MXFP4 weights with a handful of rows, in one launch: up to 8 activation rows of one matrix, or up to
-// 32 (token, expert) pairs. Formats and layouts: lp_mx.cu, the instruction: lp_mx_gemm.cu.
+// 32 (token, expert) pairs. Formats and layouts: lp_mx.cu, the instruction: lp_mx_mma.cuh.
 //
 // Bound by the weights' way from memory (0.53 bytes a value) and, where they are few, by latencies: a launch, the first copy, the last
 // sums. So there is no quantizer launch - the rows are quantized by four warps of every CTA, a 128-value step ahead of the tensor
@@ -48,11 +48,6 @@ struct SmallArgs {
     int            M, N, K, kts, rts, experts, x_rows, stages, slot_tok;      // slot_tok: tokens that a receiving slot holds
     int*           err;
 };
-
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
-__device__ __forceinline__ void arrive_release(uint32_t remote_bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(remote_bar) : "memory"); }
-__device__ __forceinline__ void st_cluster(uint32_t addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" :: "r"(addr), "f"(v) : "memory"); }
 
 template <int C, bool GROUPED>
 __global__ void __launch_bounds__(THREADS, 2) mx_small_kernel(const __grid_constant__ CUtensorMap map, const SmallArgs a) {
