@@ -180,52 +180,57 @@ __global__ void __launch_bounds__(256) mx_act_kernel(const float* __restrict__ x
 }
 
 // ---- pairs -> places in the image and a table of token tiles --------------------------------------------------------
-// One block. Every warp has a run of the pairs and counts them by expert; the counts, summed over the warps before it, are where its pairs
-// of an expert begin, so that a pair's place is by its number and not by timing. An expert gets whole groups of 8 rows of the image
-// and token tiles of its own. (A warp per expert walking all pairs: 158 us for 16,384 pairs and 128 experts, 32 of them to a block.)
-__device__ __forceinline__ int pair_expert_of(const int* pair_expert, const int* pair_row, int p, int P, int E, int x_rows) {
-    // no branch, so that the loads of several pairs are under way at once
-    const int q = p < P ? p : P - 1, e = __ldg(pair_expert + q), r = pair_row ? __ldg(pair_row + q) : 0;
-    const bool bad = e >= E || (pair_row && static_cast<unsigned>(r) >= static_cast<unsigned>(x_rows));
-    return p >= P || e < 0 ? -1 : bad ? -2 : e;
-}
-__global__ void __launch_bounds__(1024) mx_group_kernel(const int* __restrict__ pair_expert, const int* __restrict__ pair_row, int P, int E, int x_rows, int tile_w, int tile_groups,
-                                                        int2* __restrict__ place, int* __restrict__ out_row, int4* __restrict__ tab, int4* __restrict__ work, int row_tiles, int kts, int n, int* err) {
+// A block per expert (or a few). Every block counts all pairs by expert, so that it knows where its own begins: an expert gets whole groups of
+// 8 rows of the image and token tiles of its own. Its warps then have a run of the pairs each, count the expert's among them and, with the
+// counts of the warps before them, give every one its place - by its number, not by timing. 16,384 pairs, 128 experts: one block that
+// does it for all of them with match instructions 27 us, a warp per expert 158 us, so XX us.
+constexpr int GROUP_THREADS = 1024;
+constexpr int IDS_MAX = 49152;             // pairs whose experts fit into shared memory (16 bits each)
+__global__ void __launch_bounds__(GROUP_THREADS) mx_group_kernel(const int* __restrict__ pair_expert, const int* __restrict__ pair_row, int P, int E, int x_rows, int tile_w, int tile_groups,
+                                                                 int2* __restrict__ place, int* __restrict__ out_row, int4* __restrict__ tab, int4* __restrict__ work, int row_tiles, int kts,
+                                                                 int n, int* err) {
     extern __shared__ int sm[];
-    const int W = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int* start = sm;                       // first row of an expert in the image
-    int* tile0 = sm + E;                   // its first token tile
-    int* count = sm + 2 * E;               // [W][E]: the warp's pairs of an expert, then where they begin among the expert's
-    for (int i = threadIdx.x; i < W * E; i += blockDim.x) count[i] = 0;
+    __shared__ int before[GROUP_THREADS / 32];
+    int* count = sm;
+    int* start = sm + E;                   // first row of an expert in the image
+    int* tile0 = sm + 2 * E;               // its first token tile
+    uint16_t* ids = reinterpret_cast<uint16_t*>(sm + 3 * E);
+    const bool kept = P <= IDS_MAX;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int i = threadIdx.x; i < E; i += GROUP_THREADS) count[i] = 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     __syncthreads();
-    const int run = ((P + W - 1) / W + 31) & ~31, p0 = warp * run, p1 = min(p0 + run, P);
-    int* mine = count + warp * E;
-    const unsigned before = (1u << lane) - 1;
-    constexpr int U = 8;                   // loads of so many steps at once
-    for (int q = p0; q < p1; q += 32 * U) {
+    // expert of a pair; 0xffff: another GPU's, or a bad index
+    auto expert_of = [&](int p, bool& bad) {
+        // (no branch, so that the loads of several pairs are under way at once)
+        const int q = p < P ? p : P - 1, e = __ldg(pair_expert + q), r = pair_row ? __ldg(pair_row + q) : 0;
+        bad = p < P && e >= 0 && (e >= E || (pair_row && static_cast<unsigned>(r) >= static_cast<unsigned>(x_rows)));
+        return p >= P || e < 0 || bad ? 0xffff : e;
+    };
+    constexpr int U = 8;
+    for (int q = threadIdx.x; q < P; q += U * GROUP_THREADS) {
         int e[U];
+        bool bad[U];
 #pragma unroll
-        for (int i = 0; i < U; ++i) e[i] = pair_expert_of(pair_expert, pair_row, q + 32 * i + lane, p1, E, x_rows);
+        for (int i = 0; i < U; ++i) e[i] = expert_of(q + i * GROUP_THREADS, bad[i]);
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            const unsigned same = __match_any_sync(0xffffffffu, e[i]);
-            if (e[i] >= 0 && !(same & before)) mine[e[i]] += __popc(same);
-            __syncwarp();
+            const int p = q + i * GROUP_THREADS;
+            if (p >= P) break;
+            if (kept) ids[p] = static_cast<uint16_t>(e[i]);
+            if (e[i] != 0xffff) atomicAdd(count + e[i], 1);
+            else if (blockIdx.x == 0) {
+                place[p] = make_int2(-1, -1);
+                if (bad[i]) atomicCAS(err, DEV_OK, DEV_BAD_INDEX);
+            }
         }
-    }
-    __syncthreads();
-    for (int e = threadIdx.x; e < E; e += blockDim.x) {
-        int sum = 0;
-        for (int v = 0; v < W; ++v) { const int c = count[v * E + e]; count[v * E + e] = sum; sum += c; }
-        start[e] = sum;
     }
     __syncthreads();
     if (warp == 0) {
         int rows = 0, tiles = 0;
         for (int e0 = 0; e0 < E; e0 += 32) {
-            const int c = e0 + lane < E ? start[e0 + lane] : 0;
+            const int c = e0 + lane < E ? count[e0 + lane] : 0;
             const int r = (c + 7) & ~7, t = (c + tile_w - 1) / tile_w;
             int ri = r, ti = t;
 #pragma unroll
@@ -233,51 +238,52 @@ __global__ void __launch_bounds__(1024) mx_group_kernel(const int* __restrict__ 
                 const int a = __shfl_up_sync(0xffffffffu, ri, o), b = __shfl_up_sync(0xffffffffu, ti, o);
                 if (lane >= o) { ri += a; ti += b; }
             }
-            if (e0 + lane < E) {
-                const int s = rows + ri - r, t0 = tiles + ti - t;
-                start[e0 + lane] = s;
-                tile0[e0 + lane] = t0;
-                for (int i = 0; i < t; ++i) tab[t0 + i] = make_int4(e0 + lane, s + i * tile_w, min(tile_w, c - i * tile_w), (t0 + i) * tile_groups);
-            }
+            if (e0 + lane < E) { start[e0 + lane] = rows + ri - r; tile0[e0 + lane] = tiles + ti - t; }
             rows += __shfl_sync(0xffffffffu, ri, 31);
             tiles += __shfl_sync(0xffffffffu, ti, 31);
         }
-        // how the tiles are shared out (cut_of): a number of parts per lane
-        const int all = tiles * row_tiles, most = most_parts(all, kts, n);
-        const int best = __reduce_min_sync(0xffffffffu, lane < most ? cut_cost(kts, lane + 1) * MAX_PARTS + lane : 0x7fffffff);
-        const Cut c = cut_of(all, kts, n, best % MAX_PARTS + 1, best / MAX_PARTS);
-        if (lane == 0) *work = make_int4(c.tiles, c.cut, c.ctas, 0);
+        if (blockIdx.x == 0) {
+            // how the tiles are shared out (cut_of): a number of parts per lane
+            const int all = tiles * row_tiles, most = most_parts(all, kts, n);
+            const int best = __reduce_min_sync(0xffffffffu, lane < most ? cut_cost(kts, lane + 1) * MAX_PARTS + lane : 0x7fffffff);
+            const Cut c = cut_of(all, kts, n, best % MAX_PARTS + 1);
+            if (lane == 0) *work = make_int4(c.tiles, c.cut, c.ctas, 0);
+        }
     }
     __syncthreads();
-    for (int q = p0; q < p1; q += 32 * U) {
-        int e[U];
-#pragma unroll
-        for (int i = 0; i < U; ++i) e[i] = pair_expert_of(pair_expert, pair_row, q + 32 * i + lane, p1, E, x_rows);
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const int p = q + 32 * i + lane;
-            const unsigned same = __match_any_sync(0xffffffffu, e[i]);
-            const int base = e[i] >= 0 ? mine[e[i]] : 0;
-            __syncwarp();
-            if (e[i] >= 0) {
-                const int r = base + __popc(same & before);
-                place[p] = make_int2(start[e[i]] + r, (tile0[e[i]] + r / tile_w) * tile_groups * 128 + r % tile_w);
-                out_row[start[e[i]] + r] = p;
-                if (!(same & before)) mine[e[i]] = base + __popc(same);
-            } else if (p < p1) {
-                place[p] = make_int2(-1, -1);
-                if (e[i] == -2) atomicCAS(err, DEV_OK, DEV_BAD_INDEX);
+    constexpr int W = GROUP_THREADS / 32;
+    const int run = ((P + W - 1) / W + 31) & ~31, p0 = warp * run, p1 = min(p0 + run, P);
+    for (int e = blockIdx.x; e < E; e += gridDim.x) {
+        const int c = count[e];
+        if (!c) continue;
+        auto mine = [&](int p) {
+            if (p >= p1) return false;
+            bool bad;
+            return (kept ? ids[p] : expert_of(p, bad)) == e;
+        };
+        int k = 0;
+#pragma unroll 4
+        for (int p = p0; p < p1; p += 32) k += __popc(__ballot_sync(0xffffffffu, mine(p + lane)));
+        __syncthreads();                   // (the counts of the expert before are read)
+        if (lane == 0) before[warp] = k;
+        __syncthreads();
+        int at = __reduce_add_sync(0xffffffffu, lane < warp ? before[lane] : 0);
+        const int s = start[e], t0 = tile0[e];
+        for (int p = p0; p < p1; p += 32) {
+            const bool m = mine(p + lane);
+            const unsigned all = __ballot_sync(0xffffffffu, m);
+            if (m) {
+                const int r = at + __popc(all & ((1u << lane) - 1));
+                place[p + lane] = make_int2(s + r, (t0 + r / tile_w) * tile_groups * 128 + r % tile_w);
+                out_row[s + r] = p + lane;
             }
-            __syncwarp();
+            at += __popc(all);
         }
+        for (int i = threadIdx.x; i * tile_w < c; i += GROUP_THREADS) tab[t0 + i] = make_int4(e, s + i * tile_w, min(tile_w, c - i * tile_w), (t0 + i) * tile_groups);
     }
 }
 constexpr int MAX_EXPERTS = 4000;
-// warps of the grouping block: 32, or as many as leave their counters room in shared memory (200 KB in all)
-int group_warps(int experts) {
-    const int w = (200 * 1024 / 4 - 2 * experts) / experts;
-    return w < 32 ? w : 32;
-}
+size_t group_smem(int pairs, int experts) { return 3 * static_cast<size_t>(experts) * sizeof(int) + (pairs <= IDS_MAX ? static_cast<size_t>(pairs) * 2 : 0); }
 
 size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
@@ -338,13 +344,13 @@ int launch_product(const float* x, int x_rows, const uint8_t* packed, const int*
         a.out_row = reinterpret_cast<int*>(ws + p.out_row);
         a.tab = reinterpret_cast<int4*>(ws + p.tab);
         a.work = reinterpret_cast<int4*>(ws + p.work);
-        const int warps = group_warps(experts);
         static bool configured = false;
         if (!configured) {
-            if ((rc = cuda_check(cudaFuncSetAttribute(mx_group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024), "mx_group shared memory"))) return rc;
+            if ((rc = cuda_check(cudaFuncSetAttribute(mx_group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(group_smem(IDS_MAX, MAX_EXPERTS))), "mx_group shared memory")))
+                return rc;
             configured = true;
         }
-        rc = launch_early(mx_group_kernel, dim3(1), warps * 32, (warps + 2) * static_cast<size_t>(experts) * sizeof(int), st, pair_expert, pair_row, rows, experts, x_rows, p.tile_w,
+        rc = launch_early(mx_group_kernel, dim3(experts < c.sm_count ? experts : c.sm_count), GROUP_THREADS, group_smem(rows, experts), st, pair_expert, pair_row, rows, experts, x_rows, p.tile_w,
                           p.tile_groups, place, reinterpret_cast<int*>(ws + p.out_row), reinterpret_cast<int4*>(ws + p.tab), reinterpret_cast<int4*>(ws + p.work), p.row_tiles, p.kts, units, c.d_err);
         c.launches++;
         if (rc) return rc;
@@ -356,7 +362,7 @@ int launch_product(const float* x, int x_rows, const uint8_t* packed, const int*
             int parts = 1;
             for (int q = 2; q <= most; ++q)
                 if (cut_cost(p.kts, q) < cut_cost(p.kts, parts)) parts = q;
-            a.dense = cut_of(a.dense.tiles, p.kts, units, parts, cut_cost(p.kts, parts));
+            a.dense = cut_of(a.dense.tiles, p.kts, units, parts);
         }
     }
     const long long warps = static_cast<long long>(rows) * ((p.kts + 1) / 2);

@@ -18,18 +18,21 @@ struct ActDst { uint8_t* img; uint8_t* sf; int rows, groups, tile_w, tile_groups
 
 // Tiles of 256 weight rows x 256 tokens over n pairs of SMs: `cut` of `tiles` are cut, over `ctas` pairs.
 struct Cut { int tiles, cut, ctas; };
-// What a cut costs, in k steps of a whole tile (512 cycles): once, and for every part of a tile that is read back (128 KB a CTA).
+// What a cut costs where nothing comes after it, in k steps of a whole tile (512 cycles): once, and for every part of a tile that is read back.
 constexpr int CUT_COST = 14, PIECE_COST = 6;
 __host__ __device__ inline int cut_cost(int kts, int parts) { return parts == 1 ? kts : (kts + parts - 1) / parts + CUT_COST + (parts - 1) * PIECE_COST; }
 constexpr int MAX_PARTS = 32;
-// The tiles behind the last whole round are a round of their own, or each of them is cut in `parts` parts (the number that costs least, and
-// its cost), or they and the last whole round are cut over all n.
-__host__ __device__ inline Cut cut_of(int tiles, int kts, int n, int parts, int cost) {
+// Tiles that do not make a round of n. Where whole rounds follow they go first, cut over all pairs: their sums are joined during the whole tiles
+// (a part of 128 KB a CTA takes as long as some eight steps). Where there is no whole round, each is cut in `parts` parts, the number that costs least.
+__host__ __device__ inline Cut cut_of(int tiles, int kts, int n, int parts) {
     Cut c{tiles, 0, 0};
     const int left = tiles % n;
     if (!left) return c;
-    if (parts > 1) { c.cut = left; c.ctas = left * parts; }
-    if (tiles > n && static_cast<int>((static_cast<long long>(left) * kts + n - 1) / n) + CUT_COST + PIECE_COST < cost) { c.cut = left + n; c.ctas = n; }
+    if (tiles > n) parts = 1 + kts / 8;
+    const long long most = static_cast<long long>(left) * parts;
+    c.ctas = most < n ? static_cast<int>(most) : n;
+    if (c.ctas > left) c.cut = left;
+    else c.ctas = 0;
     return c;
 }
 __host__ __device__ inline int most_parts(int tiles, int kts, int n) {
