@@ -145,152 +145,215 @@ __global__ void __launch_bounds__(512) mxfp4_pack_kernel(const uint8_t* __restri
 __global__ void mxfp4_packed_kernel() {}
 
 // ---- fp32 rows -> MXFP8 image -------------------------------------------------------------------------------------
-// A warp takes 256 values of a row: a 32-value block per 4 lanes. GROUPED: the row of x and the place in the image by pair.
-template <bool GROUPED>
-__global__ void __launch_bounds__(256) mx_act_kernel(const float* __restrict__ x, int K, int kts, int rows, ActDst d, const int* __restrict__ pair_row, const int2* __restrict__ place,
-                                                     unsigned* __restrict__ counters, int n_counters) {
+// A warp takes SEGS pieces of 256 values of a row: a 32-value block per 4 lanes, all loads first. GROUPED: the row of x and the place in the image by
+// pair; a pair whose row is none of x's is taken out of the list of results and reported.
+template <bool GROUPED, int SEGS>
+__global__ void __launch_bounds__(256) mx_act_kernel(const float* __restrict__ x, int x_rows, int K, int kts, int rows, ActDst d, const int* __restrict__ pair_row,
+                                                     const int2* __restrict__ place, int* __restrict__ out_row, unsigned* __restrict__ counters, int n_counters, int* err) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int lane = threadIdx.x & 31, segs = (kts + 1) >> 1;
+    const int lane = threadIdx.x & 31, per_row = (kts + 2 * SEGS - 1) / (2 * SEGS);
     const long long id = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
     if (blockIdx.x == 0)
         for (int i = threadIdx.x; i < n_counters; i += 256) counters[i] = 0;
-    const int row = static_cast<int>(id / segs), seg = static_cast<int>(id % segs);
+    const int row = static_cast<int>(id / per_row), seg = static_cast<int>(id % per_row) * SEGS;
     if (row >= rows) return;
     int src = row, dst = row, at;                  // at: row in the groups of scales
     if (GROUPED) {
         const int2 p = place[row];
+        if (pair_row) src = pair_row[row];
         dst = p.x; at = p.y;
         if (dst < 0) return;
-        if (pair_row) src = pair_row[row];
+        if (static_cast<unsigned>(src) >= static_cast<unsigned>(x_rows)) {
+            if (lane == 0 && seg == 0) { out_row[dst] = -1; atomicCAS(err, DEV_OK, DEV_BAD_INDEX); }
+            return;
+        }
     } else {
         at = row / d.tile_w * (d.tile_groups * 128) + row % d.tile_w;
     }
-    const int k = seg * 256 + lane * 8;
-    float v[8] = {};
-    if (k < K) load8(x + static_cast<size_t>(src) * K + k, v);         // K is a multiple of 32: all eight or none
-    uint32_t sc;
-    const uint2 q = mxfp8_block8(v, lane, sc);
-    const int kt = seg * 2 + (lane >> 4);
-    if (kt >= kts) return;
-    const int piece = (lane & 15) >> 1;
-    *reinterpret_cast<uint2*>(d.img + (static_cast<size_t>(kt) * d.rows + dst) * 128 + ((piece ^ (dst & 7)) << 4) + (lane & 1) * 8) = q;
-    if ((lane & 15) == 0)
-        *reinterpret_cast<uint32_t*>(d.sf + (static_cast<size_t>(kt) * d.groups + (at >> 7)) * SF_TILE + (at & 31) * 16 + ((at >> 5) & 3) * 4) = sc;
+    const float* xr = x + static_cast<size_t>(src) * K + lane * 8;
+    float v[SEGS][8] = {};
+#pragma unroll
+    for (int i = 0; i < SEGS; ++i)
+        if ((seg + i) * 256 + lane * 8 < K) load8(xr + (seg + i) * 256, v[i]);         // K is a multiple of 32: all eight or none
+#pragma unroll
+    for (int i = 0; i < SEGS; ++i) {
+        if ((seg + i) * 2 >= kts) break;
+        uint32_t sc;
+        const uint2 q = mxfp8_block8(v[i], lane, sc);
+        const int kt = (seg + i) * 2 + (lane >> 4), piece = (lane & 15) >> 1;
+        if (kt < kts) {
+            *reinterpret_cast<uint2*>(d.img + (static_cast<size_t>(kt) * d.rows + dst) * 128 + ((piece ^ (dst & 7)) << 4) + (lane & 1) * 8) = q;
+            if ((lane & 15) == 0)
+                *reinterpret_cast<uint32_t*>(d.sf + (static_cast<size_t>(kt) * d.groups + (at >> 7)) * SF_TILE + (at & 31) * 16 + ((at >> 5) & 3) * 4) = sc;
+        }
+    }
+}
+// pieces a warp takes: four where there are enough rows to keep the SMs busy all the same (64 warps each)
+template <bool GROUPED, class... A>
+int launch_act(long long rows, int kts, cudaStream_t st, A... args) {
+    const long long segs = rows * ((kts + 1) / 2);
+    if (segs > 64ll * ctx().sm_count) return launch_early(mx_act_kernel<GROUPED, 4>, dim3(static_cast<unsigned>((rows * ((kts + 7) / 8) + 7) / 8)), 256, 0, st, args...);
+    return launch_early(mx_act_kernel<GROUPED, 1>, dim3(static_cast<unsigned>((segs + 7) / 8)), 256, 0, st, args...);
 }
 
 // ---- pairs -> places in the image and a table of token tiles --------------------------------------------------------
-// A block per expert (or a few). Every block counts all pairs by expert, so that it knows where its own begins: an expert gets whole groups of
-// 8 rows of the image and token tiles of its own. Its warps then have a run of the pairs each, count the expert's among them and, with the
-// counts of the warps before them, give every one its place - by its number, not by timing. 16,384 pairs, 128 experts: one block that
-// does it for all of them with match instructions 27 us, a warp per expert 158 us, so XX us.
+// A block per expert (or a few). With all experts' counts it knows where its own begins: each gets whole groups of 8 rows of the image and token tiles
+// of its own. Its warps have a run of the pairs each, and with the counts of the warps before them they give every pair its place - by
+// its number, not by timing. The counts are made by every block for itself (shared-memory atomics) or, from COUNT_FROM pairs on, by a launch
+// of their own. 2,048 / 16,384 pairs, 128 experts, us under ncu: a warp per expert, 32 of them to a block 24 / 158, one block with match
+// instructions 12 / 27, counts by every block 7.4 / 19, by a launch 14 / 19, XX.
 constexpr int GROUP_THREADS = 1024;
-constexpr int IDS_MAX = 49152;             // pairs whose experts fit into shared memory (16 bits each)
-__global__ void __launch_bounds__(GROUP_THREADS) mx_group_kernel(const int* __restrict__ pair_expert, const int* __restrict__ pair_row, int P, int E, int x_rows, int tile_w, int tile_groups,
-                                                                 int2* __restrict__ place, int* __restrict__ out_row, int4* __restrict__ tab, int4* __restrict__ work, int row_tiles, int kts,
-                                                                 int n, int* err) {
+constexpr int NO_EXPERT = -1, BAD_EXPERT = -2;
+__device__ __forceinline__ int expert_of(const int* __restrict__ pair_expert, int p, int P, int E) {
+    int e = NO_EXPERT;
+    if (p < P) e = __ldg(pair_expert + p);
+    return e < 0 ? NO_EXPERT : e >= E ? BAD_EXPERT : e;
+}
+__global__ void __launch_bounds__(GROUP_THREADS) mx_count_kernel(const int* __restrict__ pair_expert, int P, int E, int2* __restrict__ place,
+                                                                 int* __restrict__ counts, int* err) {
+    __shared__ int part[GROUP_THREADS / 32];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int mine = blockIdx.x; mine < E; mine += gridDim.x) {
+        int k = 0;
+        constexpr int U = 8;
+        for (int q = threadIdx.x; q < P; q += U * GROUP_THREADS) {
+            int e[U];
+#pragma unroll
+            for (int i = 0; i < U; ++i) e[i] = expert_of(pair_expert, q + i * GROUP_THREADS, P, E);
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                k += e[i] == mine;
+                if (mine == 0 && e[i] < 0 && q + i * GROUP_THREADS < P) {
+                    place[q + i * GROUP_THREADS] = make_int2(-1, -1);
+                    if (e[i] == BAD_EXPERT) atomicCAS(err, DEV_OK, DEV_BAD_INDEX);
+                }
+            }
+        }
+        k = __reduce_add_sync(0xffffffffu, k);
+        __syncthreads();
+        if (lane == 0) part[warp] = k;
+        __syncthreads();
+        if (warp == 0) {
+            k = __reduce_add_sync(0xffffffffu, part[lane]);
+            if (lane == 0) counts[mine] = k;
+        }
+    }
+}
+constexpr int COUNT_FROM = 4097;
+__global__ void __launch_bounds__(GROUP_THREADS) mx_group_kernel(const int* __restrict__ pair_expert, int P, int E, int tile_w, int tile_groups,
+                                                                 const int* __restrict__ counts, int2* __restrict__ place, int* __restrict__ out_row, int4* __restrict__ tab,
+                                                                 int4* __restrict__ work, int row_tiles, int kts, int n, int* err) {
+    constexpr int U = 16;
+    const int threads = blockDim.x, W = threads >> 5;
+    __shared__ int before[GROUP_THREADS / 32], sum_rows[GROUP_THREADS / 32], sum_tiles[GROUP_THREADS / 32];
     extern __shared__ int sm[];
-    __shared__ int before[GROUP_THREADS / 32];
     int* count = sm;
     int* start = sm + E;                   // first row of an expert in the image
     int* tile0 = sm + 2 * E;               // its first token tile
-    uint16_t* ids = reinterpret_cast<uint16_t*>(sm + 3 * E);
-    const bool kept = P <= IDS_MAX;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int i = threadIdx.x; i < E; i += GROUP_THREADS) count[i] = 0;
+    if (!counts)
+        for (int i = threadIdx.x; i < E; i += threads) count[i] = 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    __syncthreads();
-    // expert of a pair; 0xffff: another GPU's, or a bad index
-    auto expert_of = [&](int p, bool& bad) {
-        // (no branch, so that the loads of several pairs are under way at once)
-        const int q = p < P ? p : P - 1, e = __ldg(pair_expert + q), r = pair_row ? __ldg(pair_row + q) : 0;
-        bad = p < P && e >= 0 && (e >= E || (pair_row && static_cast<unsigned>(r) >= static_cast<unsigned>(x_rows)));
-        return p >= P || e < 0 || bad ? 0xffff : e;
-    };
-    constexpr int U = 8;
-    for (int q = threadIdx.x; q < P; q += U * GROUP_THREADS) {
-        int e[U];
-        bool bad[U];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int run = ((P + W - 1) / W + 31) & ~31, p0 = warp * run, p1 = min(p0 + run, P);
+    int x[U];                              // experts of the run's pairs; kept over everything below where they are no more than that
+    auto load = [&](int q) {
 #pragma unroll
-        for (int i = 0; i < U; ++i) e[i] = expert_of(q + i * GROUP_THREADS, bad[i]);
+        for (int i = 0; i < U; ++i) x[i] = expert_of(pair_expert, q + 32 * i + lane, p1, E);
+    };
+    const bool once = run <= 32 * U;
+    if (once) load(p0);
+    if (counts) {
+        for (int i = threadIdx.x; i < E; i += threads) count[i] = __ldg(counts + i);
+    } else {                               // (COUNT_FROM is such that the run is loaded)
+        __syncthreads();
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            const int p = q + i * GROUP_THREADS;
-            if (p >= P) break;
-            if (kept) ids[p] = static_cast<uint16_t>(e[i]);
-            if (e[i] != 0xffff) atomicAdd(count + e[i], 1);
-            else if (blockIdx.x == 0) {
+            const int p = p0 + 32 * i + lane;
+            if (x[i] >= 0) atomicAdd(count + x[i], 1);
+            else if (blockIdx.x == 0 && p < p1) {
                 place[p] = make_int2(-1, -1);
-                if (bad[i]) atomicCAS(err, DEV_OK, DEV_BAD_INDEX);
+                if (x[i] == BAD_EXPERT) atomicCAS(err, DEV_OK, DEV_BAD_INDEX);
             }
         }
     }
     __syncthreads();
-    if (warp == 0) {
-        int rows = 0, tiles = 0;
-        for (int e0 = 0; e0 < E; e0 += 32) {
-            const int c = e0 + lane < E ? count[e0 + lane] : 0;
-            const int r = (c + 7) & ~7, t = (c + tile_w - 1) / tile_w;
-            int ri = r, ti = t;
+    int rows = 0, tiles = 0;               // of the experts before
+    for (int e0 = 0; e0 < E; e0 += threads) {
+        const int e = e0 + threadIdx.x, c = e < E ? count[e] : 0;
+        const int r = (c + 7) & ~7, t = (c + tile_w - 1) / tile_w;
+        int ri = r, ti = t;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int a = __shfl_up_sync(0xffffffffu, ri, o), b = __shfl_up_sync(0xffffffffu, ti, o);
-                if (lane >= o) { ri += a; ti += b; }
-            }
-            if (e0 + lane < E) { start[e0 + lane] = rows + ri - r; tile0[e0 + lane] = tiles + ti - t; }
-            rows += __shfl_sync(0xffffffffu, ri, 31);
-            tiles += __shfl_sync(0xffffffffu, ti, 31);
+        for (int o = 1; o < 32; o <<= 1) {
+            const int a = __shfl_up_sync(0xffffffffu, ri, o), b = __shfl_up_sync(0xffffffffu, ti, o);
+            if (lane >= o) { ri += a; ti += b; }
         }
-        if (blockIdx.x == 0) {
-            // how the tiles are shared out (cut_of): a number of parts per lane
-            const int all = tiles * row_tiles, most = most_parts(all, kts, n);
-            const int best = __reduce_min_sync(0xffffffffu, lane < most ? cut_cost(kts, lane + 1) * MAX_PARTS + lane : 0x7fffffff);
-            const Cut c = cut_of(all, kts, n, best % MAX_PARTS + 1);
-            if (lane == 0) *work = make_int4(c.tiles, c.cut, c.ctas, 0);
+        if (lane == 31) { sum_rows[warp] = ri; sum_tiles[warp] = ti; }
+        __syncthreads();
+        const int wr = lane < W ? sum_rows[lane] : 0, wt = lane < W ? sum_tiles[lane] : 0;
+        if (e < E) {
+            start[e] = rows + ri - r;
+            tile0[e] = tiles + ti - t;
         }
+        const int br = __reduce_add_sync(0xffffffffu, lane < warp ? wr : 0), bt = __reduce_add_sync(0xffffffffu, lane < warp ? wt : 0);
+        if (e < E) { start[e] += br; tile0[e] += bt; }
+        rows += __reduce_add_sync(0xffffffffu, wr);
+        tiles += __reduce_add_sync(0xffffffffu, wt);
+        __syncthreads();
     }
-    __syncthreads();
-    constexpr int W = GROUP_THREADS / 32;
-    const int run = ((P + W - 1) / W + 31) & ~31, p0 = warp * run, p1 = min(p0 + run, P);
+    if (blockIdx.x == 0 && warp == 0) {
+        // how the tiles are shared out (cut_of): a number of parts per lane
+        const int all = tiles * row_tiles, most = most_parts(all, kts, n);
+        const int best = __reduce_min_sync(0xffffffffu, lane < most ? cut_cost(kts, lane + 1) * MAX_PARTS + lane : 0x7fffffff);
+        const Cut c = cut_of(all, kts, n, best % MAX_PARTS + 1);
+        if (lane == 0) *work = make_int4(c.tiles, c.cut, c.ctas, 0);
+    }
     for (int e = blockIdx.x; e < E; e += gridDim.x) {
         const int c = count[e];
         if (!c) continue;
-        auto mine = [&](int p) {
-            if (p >= p1) return false;
-            bool bad;
-            return (kept ? ids[p] : expert_of(p, bad)) == e;
-        };
         int k = 0;
-#pragma unroll 4
-        for (int p = p0; p < p1; p += 32) k += __popc(__ballot_sync(0xffffffffu, mine(p + lane)));
-        __syncthreads();                   // (the counts of the expert before are read)
+        for (int q = p0; q < p1; q += 32 * U) {
+            if (!once) load(q);
+#pragma unroll
+            for (int i = 0; i < U; ++i) k += x[i] == e;
+        }
+        k = __reduce_add_sync(0xffffffffu, k);
+        __syncthreads();                   // (what the expert before left there is read)
         if (lane == 0) before[warp] = k;
         __syncthreads();
         int at = __reduce_add_sync(0xffffffffu, lane < warp ? before[lane] : 0);
         const int s = start[e], t0 = tile0[e];
-        for (int p = p0; p < p1; p += 32) {
-            const bool m = mine(p + lane);
-            const unsigned all = __ballot_sync(0xffffffffu, m);
-            if (m) {
-                const int r = at + __popc(all & ((1u << lane) - 1));
-                place[p + lane] = make_int2(s + r, (t0 + r / tile_w) * tile_groups * 128 + r % tile_w);
-                out_row[s + r] = p + lane;
+        for (int q = p0; q < p1; q += 32 * U) {
+            if (!once) load(q);
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                if (q + 32 * i >= p1) break;
+                const unsigned all = __ballot_sync(0xffffffffu, x[i] == e);
+                if (x[i] == e) {
+                    const int r = at + __popc(all & ((1u << lane) - 1)), p = q + 32 * i + lane;
+                    place[p] = make_int2(s + r, (t0 + r / tile_w) * tile_groups * 128 + r % tile_w);
+                    out_row[s + r] = p;
+                }
+                at += __popc(all);
             }
-            at += __popc(all);
         }
-        for (int i = threadIdx.x; i * tile_w < c; i += GROUP_THREADS) tab[t0 + i] = make_int4(e, s + i * tile_w, min(tile_w, c - i * tile_w), (t0 + i) * tile_groups);
+        for (int i = threadIdx.x; i * tile_w < c; i += threads) tab[t0 + i] = make_int4(e, s + i * tile_w, min(tile_w, c - i * tile_w), (t0 + i) * tile_groups);
     }
 }
-constexpr int MAX_EXPERTS = 4000;
-size_t group_smem(int pairs, int experts) { return 3 * static_cast<size_t>(experts) * sizeof(int) + (pairs <= IDS_MAX ? static_cast<size_t>(pairs) * 2 : 0); }
+// threads of the grouping block: the instructions of all its warps are what the launch waits for (1024 for 2,048 pairs: 8.7 us, XX)
+int group_threads(int pairs) { return pairs < COUNT_FROM ? 256 : GROUP_THREADS; }
+static_assert(COUNT_FROM - 1 <= 256 * 16, "a warp's run of pairs is counted from registers");
+constexpr int MAX_EXPERTS = 4000;          // three words each in the 48 KB of shared memory that a launch may have without asking
 
 size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
 // What a call keeps in its workspace, and where.
 struct Plan {
     int    kts, rts, row_tiles, img_rows, groups, nt, tile_w, tile_groups, tiles_m, max_tiles, n_counters;
-    size_t img, sf, counters, part, place, out_row, tab, work, bytes;
+    size_t img, sf, counters, part, place, out_row, tab, work, counts, bytes;
 };
 Plan plan_of(int rows, int experts, int K, int N) {
     Plan p{};
@@ -319,6 +382,7 @@ Plan plan_of(int rows, int experts, int K, int N) {
         p.out_row = take(static_cast<size_t>(p.img_rows) * 4);
         p.tab = take(static_cast<size_t>(p.max_tiles) * sizeof(int4));
         p.work = take(sizeof(int4));
+        p.counts = take(static_cast<size_t>(experts) * 4);
     }
     p.bytes = at;
     return p;
@@ -344,14 +408,16 @@ int launch_product(const float* x, int x_rows, const uint8_t* packed, const int*
         a.out_row = reinterpret_cast<int*>(ws + p.out_row);
         a.tab = reinterpret_cast<int4*>(ws + p.tab);
         a.work = reinterpret_cast<int4*>(ws + p.work);
-        static bool configured = false;
-        if (!configured) {
-            if ((rc = cuda_check(cudaFuncSetAttribute(mx_group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(group_smem(IDS_MAX, MAX_EXPERTS))), "mx_group shared memory")))
-                return rc;
-            configured = true;
+        const dim3 grid(experts < c.sm_count ? experts : c.sm_count);
+        int* counts = reinterpret_cast<int*>(ws + p.counts);
+        if (rows >= COUNT_FROM) {
+            rc = launch_early(mx_count_kernel, grid, GROUP_THREADS, 0, st, pair_expert, rows, experts, place, counts, c.d_err);
+            c.launches++;
+            if (rc) return rc;
         }
-        rc = launch_early(mx_group_kernel, dim3(experts < c.sm_count ? experts : c.sm_count), GROUP_THREADS, group_smem(rows, experts), st, pair_expert, pair_row, rows, experts, x_rows, p.tile_w,
-                          p.tile_groups, place, reinterpret_cast<int*>(ws + p.out_row), reinterpret_cast<int4*>(ws + p.tab), reinterpret_cast<int4*>(ws + p.work), p.row_tiles, p.kts, units, c.d_err);
+        rc = launch_early(mx_group_kernel, grid, group_threads(rows), 3 * static_cast<size_t>(experts) * sizeof(int), st, pair_expert, rows, experts, p.tile_w, p.tile_groups,
+                          static_cast<const int*>(rows >= COUNT_FROM ? counts : nullptr), place, reinterpret_cast<int*>(ws + p.out_row), reinterpret_cast<int4*>(ws + p.tab),
+                          reinterpret_cast<int4*>(ws + p.work), p.row_tiles, p.kts, units, c.d_err);
         c.launches++;
         if (rc) return rc;
     }
@@ -365,9 +431,8 @@ int launch_product(const float* x, int x_rows, const uint8_t* packed, const int*
             a.dense = cut_of(a.dense.tiles, p.kts, units, parts);
         }
     }
-    const long long warps = static_cast<long long>(rows) * ((p.kts + 1) / 2);
-    rc = launch_early(mx_act_kernel<GROUPED>, dim3(static_cast<unsigned>((warps + 7) / 8)), 256, 0, st, x, K, p.kts, rows, ActDst{ws + p.img, ws + p.sf, p.img_rows, p.groups, p.tile_w, p.tile_groups},
-                      pair_row, static_cast<const int2*>(place), reinterpret_cast<unsigned*>(ws + p.counters), p.n_counters);
+    rc = launch_act<GROUPED>(rows, p.kts, st, x, x_rows, K, p.kts, rows, ActDst{ws + p.img, ws + p.sf, p.img_rows, p.groups, p.tile_w, p.tile_groups}, pair_row, static_cast<const int2*>(place),
+                             GROUPED ? reinterpret_cast<int*>(ws + p.out_row) : nullptr, reinterpret_cast<unsigned*>(ws + p.counters), p.n_counters, c.d_err);
     c.launches++;
     if (rc) return rc;
     CUtensorMap map;

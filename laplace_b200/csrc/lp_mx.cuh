@@ -48,7 +48,7 @@ struct MxArgs {
     float*         y;
     int            M, N, kts, rts, img_rows, groups, tile_w;
     int            tile_groups;  // 128-row groups of scales of a token tile
-    // experts: {expert, first row in the image, rows, first group} of every token tile, their number, and the pair of every image row
+    // experts: {expert, first row in the image, rows, first group} of every token tile, their number, and the pair of every image row (-1: a bad one)
     const int4*    tab;
     const int4*    work;         // {row tiles of all token tiles, how many of them are cut, over how many units, -}
     const int*     out_row;

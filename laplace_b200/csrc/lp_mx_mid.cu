@@ -169,12 +169,12 @@ __global__ void __launch_bounds__(THREADS, 1) mx_mid_kernel(const __grid_constan
                     const int c0 = 32 * half + 64 * j, here = min(32, s.n - c0);
                     if (here <= 0) break;
                     if (GROUPED) {
-                        // lane: the row of y that column c0 + lane goes to
+                        // lane: the row of y that column c0 + lane goes to, -1: to none
                         const int to = lane < here ? __ldg(a.out_row + s.row0 + c0 + lane) : 0;
 #pragma unroll
                         for (int k = 0; k < 32; ++k) {
                             const int m = __shfl_sync(0xffffffffu, to, k);
-                            if (k < here && col < a.N) a.y[static_cast<size_t>(m) * a.N + col] = v[j][k];
+                            store_if(k < here && m >= 0 && col < a.N, a.y + static_cast<size_t>(m) * a.N + col, v[j][k]);
                         }
                     } else if (col < a.N) {
                         float* q = a.y + static_cast<size_t>(c0) * a.N + col;
@@ -216,8 +216,9 @@ __global__ void __launch_bounds__(THREADS, 1) mx_mid_kernel(const __grid_constan
                 const float e[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const int m = m0 + 4 * g + k;
-                    if (4 * g + k < mine && col < a.N) a.y[static_cast<size_t>(GROUPED ? __ldg(a.out_row + s.row0 + m) : m) * a.N + col] = e[k];
+                    if (4 * g + k >= mine) break;
+                    const int m = m0 + 4 * g + k, to = GROUPED ? __ldg(a.out_row + s.row0 + m) : m;
+                    if (to >= 0 && col < a.N) a.y[static_cast<size_t>(to) * a.N + col] = e[k];
                 }
             }
             if (t + clusters < tiles) {             // there is a next tile: the buffer is free for every CTA

@@ -43,6 +43,10 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, float v) { asm volatil
 __device__ __forceinline__ void st_cluster4(uint32_t addr, float a, float b, float c, float d) {
     asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" :: "r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
+// *p = v where `on`, without a branch (with one the 32 stores of a column block no longer overlap: experts' products 36 -> 61 us)
+__device__ __forceinline__ void store_if(bool on, float* p, float v) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p st.global.f32 [%0], %1;\n\t}" :: "l"(p), "f"(v), "r"(static_cast<uint32_t>(on)) : "memory");
+}
 // 32 lanes x 8 columns
 __device__ __forceinline__ void ld8(uint32_t taddr, float (&v)[8]) {
     uint32_t r[8];

@@ -312,12 +312,12 @@ __global__ void __launch_bounds__(THREADS, 1) mx_pair_kernel(const __grid_consta
                 const int c0 = 32 * half + 64 * j, here = min(32, s.n - c0);
                 if (here <= 0) break;
                 if (GROUPED) {
-                    // lane: the row of y that column c0 + lane goes to
+                    // lane: the row of y that column c0 + lane goes to, -1: to none
                     const int to = lane < here ? __ldg(a.out_row + s.row0 + c0 + lane) : 0;
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         const int m = __shfl_sync(0xffffffffu, to, i);
-                        if (i < here && col < a.N) a.y[static_cast<size_t>(m) * a.N + col] = v[j][i];
+                        store_if(i < here && m >= 0 && col < a.N, a.y + static_cast<size_t>(m) * a.N + col, v[j][i]);
                     }
                 } else if (col < a.N) {
                     float* q = a.y + static_cast<size_t>(s.row0 + c0) * a.N + col;
