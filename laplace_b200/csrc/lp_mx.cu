@@ -348,11 +348,30 @@ int group_threads(int pairs) { return pairs < COUNT_FROM ? 256 : GROUP_THREADS; 
 static_assert(COUNT_FROM - 1 <= 256 * 16, "a warp's run of pairs is counted from registers");
 constexpr int MAX_EXPERTS = 4000;          // three words each in the 48 KB of shared memory that a launch may have without asking
 
+// How the tiles of one matrix on pairs of SMs are shared out, and what that takes by the model below: cycles.
+struct Shared { Cut cut; long long cycles; };
+Shared share_out(int tiles, int width, int kts, int n) {
+    const int most = most_parts(tiles, kts, n);
+    int parts = 1;
+    for (int q = 2; q <= most; ++q)
+        if (cut_cost(kts, q) < cut_cost(kts, parts)) parts = q;
+    const Cut c = cut_of(tiles, kts, n, parts);
+    long long steps = static_cast<long long>(tiles / n) * kts;
+    if (c.cut && tiles < n) steps = cut_cost(kts, parts);
+    else if (c.cut) steps += over_cost(c.cut, kts, c.ctas);
+    else if (tiles % n) steps += kts;
+    // A step brings 16 KB of weights and 64 bytes a token into a CTA's shared memory and out again, 128 bytes a cycle; results leave at 18 cycles a
+    // token. (512 x 4096 x 4096: tiles of 256 tokens 19.4 us, of 192 17.9, of 128 16.9.)
+    return {c, steps * (256 + width) + 18ll * width};
+}
+int round32(int n) { return (n + 31) & ~31; }
+
 size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
 // What a call keeps in its workspace, and where.
 struct Plan {
     int    kts, rts, row_tiles, img_rows, groups, nt, tile_w, tile_groups, tiles_m, max_tiles, n_counters;
+    Cut    share;                  // tiles of one matrix
     size_t img, sf, counters, part, place, out_row, tab, work, counts, bytes;
 };
 Plan plan_of(int rows, int experts, int K, int N) {
@@ -363,12 +382,22 @@ Plan plan_of(int rows, int experts, int K, int N) {
     p.img_rows = static_cast<int>((most + 7) & ~7ll);
     const int per = experts ? (rows + experts - 1) / experts : rows;
     p.nt = per <= 32 ? 32 : per <= 64 ? 64 : per <= 128 ? 128 : 256;
-    p.tiles_m = (rows + p.nt - 1) / p.nt;
     const bool pairs = p.nt == 256;
     p.row_tiles = pairs ? (p.rts + 1) / 2 : p.rts;
-    p.tile_w = experts ? p.nt : ((rows + p.tiles_m - 1) / p.tiles_m + 31) & ~31;
+    p.tiles_m = (rows + p.nt - 1) / p.nt;
+    p.tile_w = p.nt;
+    p.share = Cut{p.tiles_m * p.row_tiles, 0, 0};
+    if (pairs && !experts) {
+        long long least = 1ll << 62;
+        const int first = p.tiles_m;
+        for (int m = first; m <= 4 * first && m <= first + 8; ++m) {
+            const int w = round32((rows + m - 1) / m), tiles_m = (rows + w - 1) / w;
+            const Shared s = share_out(tiles_m * p.row_tiles, w, p.kts, ctx().sm_count / 2);
+            if (s.cycles < least) { least = s.cycles; p.tiles_m = tiles_m; p.tile_w = w; p.share = s.cut; }
+        }
+    }
     p.n_counters = pairs ? mx_pair_counters() : 0;
-    p.tile_groups = (p.nt + 127) / 128;
+    p.tile_groups = (p.tile_w + 127) / 128;
     p.max_tiles = experts ? rows / p.tile_w + (experts < rows ? experts : rows) : p.tiles_m;
     p.groups = p.max_tiles * p.tile_groups;
     size_t at = 0;
@@ -421,16 +450,7 @@ int launch_product(const float* x, int x_rows, const uint8_t* packed, const int*
         c.launches++;
         if (rc) return rc;
     }
-    if (!GROUPED) {
-        a.dense = Cut{p.tiles_m * p.row_tiles, 0, 0};
-        if (p.nt == 256) {
-            const int most = most_parts(a.dense.tiles, p.kts, units);
-            int parts = 1;
-            for (int q = 2; q <= most; ++q)
-                if (cut_cost(p.kts, q) < cut_cost(p.kts, parts)) parts = q;
-            a.dense = cut_of(a.dense.tiles, p.kts, units, parts);
-        }
-    }
+    a.dense = p.share;
     rc = launch_act<GROUPED>(rows, p.kts, st, x, x_rows, K, p.kts, rows, ActDst{ws + p.img, ws + p.sf, p.img_rows, p.groups, p.tile_w, p.tile_groups}, pair_row, static_cast<const int2*>(place),
                              GROUPED ? reinterpret_cast<int*>(ws + p.out_row) : nullptr, reinterpret_cast<unsigned*>(ws + p.counters), p.n_counters, c.d_err);
     c.launches++;

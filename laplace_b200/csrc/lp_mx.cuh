@@ -22,17 +22,19 @@ struct Cut { int tiles, cut, ctas; };
 constexpr int CUT_COST = 14, PIECE_COST = 6;
 __host__ __device__ inline int cut_cost(int kts, int parts) { return parts == 1 ? kts : (kts + parts - 1) / parts + CUT_COST + (parts - 1) * PIECE_COST; }
 constexpr int MAX_PARTS = 32;
-// Tiles that do not make a round of n. Where whole rounds follow they go first, cut over all pairs: their sums are joined during the whole tiles
-// (a part of 128 KB a CTA takes as long as some eight steps). Where there is no whole round, each is cut in `parts` parts, the number that costs least.
+// Tiles that do not make a round of n. Without a whole round each is cut in `parts` parts, the number that costs least. Where whole rounds follow, the
+// tiles before them may be cut over all pairs, into parts of eight steps at least; their sums are joined during the whole tiles, but the way to
+// memory and back costs all the same (512 x 4096 x 14336, 38 tiles of 32 steps over, 74 pairs: 33.8 us cut, 31.8 whole; 2048 x 14336 x 4096,
+// 54 of 112 steps: 108 either way).
+__host__ __device__ inline int over_cost(int left, int kts, int ctas) { return static_cast<int>((static_cast<long long>(left) * kts + ctas - 1) / ctas) + CUT_COST + 3 * ctas / left; }
 __host__ __device__ inline Cut cut_of(int tiles, int kts, int n, int parts) {
     Cut c{tiles, 0, 0};
     const int left = tiles % n;
     if (!left) return c;
     if (tiles > n) parts = 1 + kts / 8;
     const long long most = static_cast<long long>(left) * parts;
-    c.ctas = most < n ? static_cast<int>(most) : n;
-    if (c.ctas > left) c.cut = left;
-    else c.ctas = 0;
+    const int ctas = most < n ? static_cast<int>(most) : n;
+    if (ctas > left && (tiles < n || over_cost(left, kts, ctas) < kts)) { c.cut = left; c.ctas = ctas; }
     return c;
 }
 __host__ __device__ inline int most_parts(int tiles, int kts, int n) {
