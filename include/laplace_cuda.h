@@ -272,8 +272,11 @@ int laplace_cuda_lm_head_dev(const float* x, const uint8_t* w, uint32_t type, fl
  *   negative expert leaves its row of y untouched; an expert >= n_experts_total or a row outside [0, x_rows) does too and
  *   makes the next laplace_cuda_sync() return LAPLACE_ERR_ARG. At most 4000 experts. n_pairs = 0 is a call without effect.
  * K is a multiple of 32, x 16-byte aligned. Workspace: the caller's, laplace_cuda_mxfp4_workspace_size(M or n_pairs, 0 or
- *   n_experts_total, K, N) bytes, 256-byte aligned, its contents of no consequence before or after. Calls with workspaces of
- *   their own may overlap, in streams as in captured graphs. Results do not depend on timing: the same call gives the same bits.
+ *   n_experts_total, K, N) bytes (after laplace_cuda_init; 0: none is needed, NULL will do, or the sizes are none that a call
+ *   takes), 256-byte aligned, its contents of no consequence before or after. Calls with workspaces of their own may overlap,
+ *   in streams as in captured graphs. Results do not depend on timing: the same call gives the same bits.
+ * Up to 8 rows of one matrix the call copies weights before it has waited for the kernel before it (see "Overlap" above); the
+ *   packed weights of laplace_cuda_mxfp4_pack_dev are safe at once.
  * All pointers are device memory. */
 int    laplace_cuda_mxfp4_quantize_dev(const void* x, uint32_t x_type, uint8_t* w, long long n, void* stream);
 size_t laplace_cuda_mxfp4_packed_size(int n_experts, int N, int K);

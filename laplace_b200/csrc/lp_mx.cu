@@ -532,7 +532,7 @@ int laplace_cuda_mxfp4_pack_dev(const uint8_t* w, uint8_t* packed, int n_experts
 }
 
 size_t laplace_cuda_mxfp4_workspace_size(int rows, int n_experts, int K, int N) {
-    if (!ctx().ready || rows <= 0 || n_experts < 0 || K <= 0 || N <= 0 || K % 32) return 0;
+    if (!ctx().ready || rows <= 0 || n_experts < 0 || K <= 0 || N <= 0 || K % 32 || mx_small_takes(rows, n_experts > 0)) return 0;
     return plan_of(rows, n_experts, K, N).bytes;
 }
 
@@ -542,10 +542,11 @@ int laplace_cuda_mxfp4_gemm_dev(const float* x, const uint8_t* packed, float* y,
     if (M < 0) return fail(LAPLACE_ERR_ARG, "mxfp4_gemm: M=%d", M);
     if (M == 0) return LAPLACE_OK;
     if (M > 1 << 24 || too_many(M, 1, N)) return fail(LAPLACE_ERR_LIMIT, "mxfp4_gemm: M=%d", M);
-    if (!x || !packed || !y || !workspace) return fail(LAPLACE_ERR_ARG, "mxfp4_gemm: null pointer");
+    const size_t need = laplace_cuda_mxfp4_workspace_size(M, 0, K, N);
+    if (!x || !packed || !y || (need && !workspace)) return fail(LAPLACE_ERR_ARG, "mxfp4_gemm: null pointer");
     if (misaligned(x, 16) || misaligned(packed, 128) || misaligned(workspace, 256) || misaligned(y, 4))
         return fail(LAPLACE_ERR_ARG, "mxfp4_gemm: x must be 16-byte, packed 128-byte, workspace 256-byte aligned");
-    if (workspace_bytes < plan_of(M, 0, K, N).bytes) return fail(LAPLACE_ERR_ARG, "mxfp4_gemm: workspace of %zu bytes, %zu needed", workspace_bytes, plan_of(M, 0, K, N).bytes);
+    if (workspace_bytes < need) return fail(LAPLACE_ERR_ARG, "mxfp4_gemm: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     return launch_product<false>(x, M, packed, nullptr, nullptr, M, 1, y, K, N, static_cast<uint8_t*>(workspace), MX_STREAM(stream));
 }
 
@@ -557,11 +558,11 @@ int laplace_cuda_mxfp4_moe_grouped_dev(const float* x, int x_rows, const uint8_t
     if (n_pairs == 0) return LAPLACE_OK;
     if (n_pairs > 1 << 24 || too_many(n_pairs, n_experts_total, N)) return fail(LAPLACE_ERR_LIMIT, "mxfp4_moe_grouped: n_pairs=%d", n_pairs);
     if (n_experts_total > MAX_EXPERTS) return fail(LAPLACE_ERR_LIMIT, "mxfp4_moe_grouped: %d experts, %d at most", n_experts_total, MAX_EXPERTS);
-    if (!x || !packed || !pair_expert || !y || !workspace) return fail(LAPLACE_ERR_ARG, "mxfp4_moe_grouped: null pointer");
+    const size_t need = laplace_cuda_mxfp4_workspace_size(n_pairs, n_experts_total, K, N);
+    if (!x || !packed || !pair_expert || !y || (need && !workspace)) return fail(LAPLACE_ERR_ARG, "mxfp4_moe_grouped: null pointer");
     if (!pair_row && x_rows < n_pairs) return fail(LAPLACE_ERR_ARG, "mxfp4_moe_grouped: %d rows of x for %d pairs", x_rows, n_pairs);
     if (misaligned(x, 16) || misaligned(packed, 128) || misaligned(workspace, 256) || misaligned(y, 4) || misaligned(pair_expert, 4) || misaligned(pair_row, 4))
         return fail(LAPLACE_ERR_ARG, "mxfp4_moe_grouped: x must be 16-byte, packed 128-byte, workspace 256-byte aligned");
-    const size_t need = plan_of(n_pairs, n_experts_total, K, N).bytes;
     if (workspace_bytes < need) return fail(LAPLACE_ERR_ARG, "mxfp4_moe_grouped: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     return launch_product<true>(x, x_rows, packed, pair_expert, pair_row, n_pairs, n_experts_total, y, K, N, static_cast<uint8_t*>(workspace), MX_STREAM(stream));
 }

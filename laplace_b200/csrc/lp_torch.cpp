@@ -288,11 +288,11 @@ PyObject* py_mxfp4_gemm(PyObject*, PyObject* const* a, Py_ssize_t n) {
             Py_RETURN_NONE;
         const at::Tensor out = y ? *y : fresh({M, N}, at::kFloat);
         const long bytes = static_cast<long>(g.mxfp4_workspace_size(M, 0, K, N));
-        const at::Tensor ws = fresh({bytes}, at::kByte);
+        const at::Tensor ws = bytes ? fresh({bytes}, at::kByte) : at::Tensor();
         const auto* px = ptr<const float>(*x);
         const auto* pw = ptr<const uint8_t>(*w);
         auto* po = ptr<float>(out);
-        void *pws = ws.data_ptr(), *st = stream();
+        void *pws = bytes ? ws.data_ptr() : nullptr, *st = stream();
         if (unlocked([&] { return g.mxfp4_gemm(px, pw, po, M, K, N, pws, bytes, st); }))
             Py_RETURN_NONE;
         if (y) { Py_INCREF(a[5]); return a[5]; }
@@ -313,12 +313,12 @@ PyObject* py_mxfp4_moe_grouped(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (P >= 1L << 31 || rows >= 1L << 31 || (y && y->numel() < P * N)) Py_RETURN_NONE;
         const at::Tensor out = y ? *y : fresh({P, N}, at::kFloat);
         const long bytes = static_cast<long>(g.mxfp4_workspace_size(P, E, K, N));
-        const at::Tensor ws = fresh({bytes}, at::kByte);
+        const at::Tensor ws = bytes ? fresh({bytes}, at::kByte) : at::Tensor();
         const auto* px = ptr<const float>(*x);
         const auto* pw = ptr<const uint8_t>(*w);
         const auto *pi = ptr<const int>(*idx), *pr = row ? ptr<const int>(*row) : nullptr;
         auto* po = ptr<float>(out);
-        void *pws = ws.data_ptr(), *st = stream();
+        void *pws = bytes ? ws.data_ptr() : nullptr, *st = stream();
         if (unlocked([&] { return g.mxfp4_moe_grouped(px, rows, pw, pi, pr, P, E, po, K, N, pws, bytes, st); }))
             Py_RETURN_NONE;
         if (y) { Py_INCREF(a[7]); return a[7]; }

@@ -53,9 +53,11 @@ def mxfp8(x):
 
 
 def product(x, w):
-    """(y, mass): y = xq . w^T and the sums of the terms' magnitudes; x fp32 [M, K], w values [N, K]."""
-    xq = mxfp8(x)
-    return xq @ w.T, np.abs(xq) @ np.abs(w).T
+    """(y, mass): y = xq . w^T and the sums of the terms' magnitudes, in 64 bits; x fp32 [M, K], w values [N, K]."""
+    import torch
+    dev = "cuda" if torch.cuda.is_available() else "cpu"
+    xq, wt = torch.from_numpy(mxfp8(x)).to(dev), torch.from_numpy(np.ascontiguousarray(w)).to(dev).t()
+    return (xq @ wt).cpu().numpy(), (xq.abs() @ wt.abs()).cpu().numpy()
 
 
 def tolerance(K, mass):

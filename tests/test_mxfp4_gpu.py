@@ -129,7 +129,7 @@ def test_pack_layout(experts, n, k, off):
 
 SHAPES = [(1, 32, 1), (1, 64, 129), (1, 4096, 1024), (2, 160, 200), (7, 288, 64), (8, 2848, 384), (9, 512, 4096), (16, 128, 128), (17, 96, 1000), (24, 14336, 256), (31, 1024, 640),
           (32, 2816, 130), (33, 4096, 512), (64, 160, 300), (65, 2048, 257), (77, 2816, 1056), (96, 544, 4000), (128, 1024, 128), (129, 4096, 384), (200, 256, 2000), (255, 352, 513),
-          (256, 4096, 1024), (257, 1056, 700), (300, 14336, 256), (512, 2048, 2816), (777, 768, 1411), (1030, 96, 2100), (2048, 512, 1024)]
+          (256, 4096, 1024), (257, 1056, 700), (300, 14336, 256), (512, 2048, 2816), (777, 768, 1411), (1030, 96, 2100), (2048, 512, 1024), (5000, 64, 300), (1200, 14336, 256), (260, 4096, 200), (9, 14336, 1000), (100, 14336, 64)]
 
 
 @pytest.mark.parametrize("M,K,N", SHAPES)
@@ -224,8 +224,9 @@ def _routing(seed, T, E, k, skew):
     return np.argsort(-logits, axis=1)[:, :k].astype(np.int32).reshape(-1)
 
 
-@pytest.mark.parametrize("T,E,k,K,N,skew", [(1, 128, 8, 2048, 1536, 0.), (1, 4, 1, 32, 1, 0.), (5, 4, 2, 160, 200, 1.), (24, 60, 4, 768, 130, 1.), (100, 8, 3, 256, 520, 2.),
-                                            (256, 32, 8, 512, 256, 1.5), (600, 4, 2, 96, 257, 1.), (700, 128, 8, 128, 96, 2.), (40, 1, 1, 288, 300, 0.)])
+@pytest.mark.parametrize("T,E,k,K,N,skew", [(1, 32, 8, 2048, 384, 0.), (1, 4, 1, 32, 1, 0.), (4, 32, 8, 352, 300, 3.), (5, 4, 2, 160, 200, 1.), (24, 60, 4, 768, 130, 1.), (100, 8, 3, 256, 520, 2.),
+                                            (256, 32, 8, 512, 256, 1.5), (600, 4, 2, 96, 257, 1.), (700, 128, 8, 128, 96, 2.), (40, 1, 1, 288, 300, 0.), (1400, 3, 2, 1056, 700, 1.),
+                                            (3000, 8, 2, 96, 130, 2.), (20000, 4, 1, 32, 40, 1.), (2000, 1500, 3, 64, 24, 2.), (700, 600, 3, 32, 33, 3.), (60000, 3, 1, 32, 8, 1.)])
 @pytest.mark.parametrize("form", ["shared", "own", "elsewhere"])
 def test_grouped(T, E, k, K, N, skew, form):
     from laplace_b200 import device
@@ -377,12 +378,21 @@ def test_refusals():
                 lambda: device.mxfp4_moe_grouped(x[:3], packed, expert, None, E, K, N), lambda: device.mxfp4_moe_grouped(x, packed, expert, None, 0, K, N)):
         with pytest.raises(LaplaceCudaError):
             bad()
-    ws = torch.empty(L.laplace_cuda_mxfp4_workspace_size(4, 0, K, N), dtype=torch.uint8, device="cuda")
-    y = torch.empty(4, N, device="cuda")
-    args = [x.data_ptr(), packed.data_ptr(), y.data_ptr(), 4, K, N, ws.data_ptr()]
+    M = 40
+    assert L.laplace_cuda_mxfp4_workspace_size(8, 0, K, N) == 0 and L.laplace_cuda_mxfp4_workspace_size(32, E, K, N) == 0       # none is needed
+    for bad in ((0, 0, K, N), (M, -1, K, N), (M, 0, 48, N), (M, 0, K, 0)):
+        assert L.laplace_cuda_mxfp4_workspace_size(*bad) == 0
+    assert L.laplace_cuda_mxfp4_packed_size(1, N, 48) == 0 and L.laplace_cuda_mxfp4_packed_size(0, N, K) == 0
+    x = _dev(_act(992, M, K))
+    ws = torch.empty(L.laplace_cuda_mxfp4_workspace_size(M, 0, K, N), dtype=torch.uint8, device="cuda")
+    y = torch.empty(M, N, device="cuda")
+    args = [x.data_ptr(), packed.data_ptr(), y.data_ptr(), M, K, N, ws.data_ptr()]
+    assert L.laplace_cuda_mxfp4_gemm_dev(*args, ws.numel(), 1) == 0
     assert L.laplace_cuda_mxfp4_gemm_dev(*args, ws.numel() - 1, 1) == -1
     assert L.laplace_cuda_mxfp4_gemm_dev(*args[:6], None, ws.numel(), 1) == -1
+    assert L.laplace_cuda_mxfp4_gemm_dev(*args[:6], ws.data_ptr() + 16, ws.numel(), 1) == -1
     assert L.laplace_cuda_mxfp4_gemm_dev(*args[:3], -1, K, N, ws.data_ptr(), ws.numel(), 1) == -1
+    assert L.laplace_cuda_mxfp4_gemm_dev(*args[:3], 1 << 25, K, N, ws.data_ptr(), ws.numel(), 1) == -5
     for i in range(3):
         assert L.laplace_cuda_mxfp4_gemm_dev(*(args[:i] + [None] + args[i + 1:]), ws.numel(), 1) == -1
     assert L.laplace_cuda_mxfp4_quantize_dev(x.data_ptr(), 2, w.data_ptr(), 32, 1) == 1
@@ -446,3 +456,54 @@ def test_native_and_general_paths_agree():
             return v.sum()
         torch.vmap(f)(x)
     device.sync()
+
+
+def test_from_a_gguf_file(tmp_path):
+    """A file's MXFP4 matrix and this GPU's half of its experts: loaded, packed, multiplied."""
+    import torch
+    from laplace_b200 import device
+    from laplace_b200.gguf import GgufFile
+    from tests.gguf_file import write_gguf
+    K, N, E, NE = 96, 300, 4, 48
+    (w, v), (we, ve) = _blocks(1300, N, K), _blocks(1301, E * NE, K)
+    path = tmp_path / "m.gguf"
+    write_gguf(path, [("general.architecture", "str", "llama")], [("norm", [K], 0, np.ones(K, dtype=np.float32).tobytes()), ("w", [K, N], 39, w.tobytes()), ("exps", [K, NE, E], 39, we.tobytes())],
+               alignment=32)
+    device.lib()
+    g = GgufFile(path, 1, 2)
+    try:
+        g.upload()
+        t, e = g.tensor("w"), g.tensor("exps")
+        rows = t.rows[1] - t.rows[0]
+        packed, experts = device.mxfp4_pack(t.as_torch(), rows, K), device.mxfp4_pack(e.as_torch(), NE, K, 2)
+        x = _act(1302, 11, K)
+        y = device.mxfp4_gemm(_dev(x), packed, 11, K, rows)
+        pick = np.arange(11, dtype=np.int32) % 3 - 1
+        z = device.mxfp4_moe_grouped(_dev(x), experts, _dev(pick), None, 2, K, NE, y=torch.zeros(11, NE, device="cuda"))
+        device.sync()
+        _close(y, *ref.product(x, v[t.rows[0]:t.rows[1]]), K)
+        _close(z, *_grouped_ref(x, ve.reshape(E, NE, K)[2:], pick, None, np.zeros((11, NE))), K)
+    finally:
+        g.close()
+
+
+def test_more_pairs_than_one_block_counts_and_bad_rows_among_them():
+    """Rows of x out of range among thousands of pairs, in each size class of the products: skipped, reported, the others right."""
+    import torch
+    from laplace_b200 import device
+    from laplace_b200.matmul import LaplaceCudaError
+    for T, E, k, K, N in ((60, 8, 2, 64, 140), (300, 4, 2, 64, 140), (2500, 4, 2, 64, 140)):
+        w, v = _blocks(1310, E * N, K)
+        expert, row = _routing(1311, T, E, k, 0.5), np.repeat(np.arange(T, dtype=np.int32), k)
+        bad = np.arange(5, T * k, 37)
+        row[bad] = np.where(bad % 2, T, -1)
+        x = _act(1312, T, K)
+        y0 = np.full((T * k, N), 7.0, dtype=np.float32)
+        y = device.mxfp4_moe_grouped(_dev(x), device.mxfp4_pack(_dev(w), N, K, E), _dev(expert), _dev(row), E, K, N, y=_dev(y0))
+        with pytest.raises(LaplaceCudaError):
+            device.sync()
+        device.sync()
+        ok = expert.copy()
+        ok[bad] = -1
+        _close(y, *_grouped_ref(x, v.reshape(E, N, K), ok, np.clip(row, 0, T - 1), y0), K, f"{T}")
+        assert torch.equal(y[torch.from_numpy(bad).cuda()], torch.full((len(bad), N), 7.0, device="cuda"))
