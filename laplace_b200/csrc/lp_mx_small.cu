@@ -2,12 +2,12 @@
 // 32 (token, expert) pairs. Formats and layouts: lp_mx.cu, the instruction: lp_mx_mma.cuh.
 //
 // Bound by the weights' way from memory (0.53 bytes a value) and, where they are few, by latencies: a launch, the first copy, the last
-// sums. So there is no quantizer launch - the rows are quantized by four warps of every CTA, a 128-value step ahead of the tensor
+// sums. So there is no quantizer launch - the rows are quantized by eight warps of every CTA, a 128-value step ahead of the tensor
 // core, out of L2 (M x 512 bytes beside 8.7 KB of weights) - and no sum goes through memory: the CTAs of a cluster share out k, and each sends its
 // part of a tile's results straight into the shared memory of the tile's owner, which adds them in the order of k and writes y.
 //
 // A cluster of C CTAs takes tiles (128 weight rows x up to 8 tokens) number cluster, cluster + clusters, ...; the i-th of them is owned by CTA i % C.
-// Roles by warp: 0 copies, 1 MMA issue (owns the TMEM), 2, 3, 8, 9 quantizers, 4-7 drain (lane = weight row), sums and output. All waits are
+// Roles by warp: 0 copies, 1 MMA issue (owns the TMEM), 2, 3, 8-13 quantizers (in pairs, four rows each), 4-7 drain (lane = weight row), sums and output. All waits are
 // bounded; a wait that gives up raises the status word and the roles leave their loops. No CTA leaves before its cluster is done.
 #include "lp_mx.cuh"
 #include "lp_mx_mma.cuh"
@@ -19,8 +19,8 @@ namespace {
 using namespace mx;
 using namespace tc;
 
-constexpr int THREADS = 320;
-constexpr int QUANT = 4;                       // quantizer warps. At most the stages: a warp that waits for a stage must have seen the use before the last one end
+constexpr int THREADS = 448;
+constexpr int QUANT = 4;                       // pairs of quantizer warps. At most the stages: a warp that waits for a stage must have seen the use before the last one end
 constexpr int TOK = 8, MAX_PAIRS = 32;
 constexpr int N_MMA = 16;                      // columns of the instruction; those from TOK on are not read
 constexpr int ACCS = 8;                        // accumulators in TMEM
@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(THREADS, 2) mx_small_kernel(const __grid_const
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = C > 1 ? static_cast<int>(pair_rank()) : 0;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < S; ++i) { mbar_init(bar(f.full[i]), 2); mbar_init(bar(f.empty[i]), 1); }
+        for (int i = 0; i < S; ++i) { mbar_init(bar(f.full[i]), 3); mbar_init(bar(f.empty[i]), 1); }
         for (int i = 0; i < ACCS; ++i) { mbar_init(bar(f.tfull[i]), 1); mbar_init(bar(f.tempty[i]), 4); }
         for (int i = 0; i < SLOTS; ++i) mbar_init(bar(f.recv[i]), 4 * C);
         for (int i = 0; i < C * SLOTS; ++i) mbar_init(bar(f.avail[i]), 4);
@@ -155,8 +155,8 @@ __global__ void __launch_bounds__(THREADS, 2) mx_small_kernel(const __grid_const
         }
         if (C > 1) cluster_wait();
     } else if (warp == 2 || warp == 3 || warp >= 8) {
-        // 16 lanes a row: a step is 128 values of two rows, 8 values a lane, a 32-value block per four lanes
-        const int which = warp < 4 ? warp - 2 : warp - 6, half = lane >> 4, k8 = (lane & 15) * 8;
+        // 16 lanes a row: a step is 128 values of two rows, 8 values a lane, a 32-value block per four lanes; the second warp of a pair has rows 4 to 7
+        const int w = warp < 4 ? warp - 2 : warp - 6, which = w >> 1, m0 = (w & 1) * (TOK / 2) + (lane >> 4), k8 = (lane & 15) * 8;
         asm volatile("griddepcontrol.wait;" ::: "memory");
         int st = 0, parity = 1, turn = 0;
         bool ok = true;
@@ -165,10 +165,10 @@ __global__ void __launch_bounds__(THREADS, 2) mx_small_kernel(const __grid_const
             for (int kt = k0; kt < k1; ++kt) {
                 if (turn == which) {
                     const int k = kt * 128 + k8;
-                    float v[TOK / 2][8];
+                    float v[TOK / 4][8];
 #pragma unroll
-                    for (int j = 0; j < TOK / 2; ++j) {            // loads of all rows before the wait and the first use
-                        const int m = 2 * j + half;
+                    for (int j = 0; j < TOK / 4; ++j) {            // loads of all rows before the wait and the first use
+                        const int m = m0 + 2 * j;
                         if (m < n && k < a.K) load8(a.x + static_cast<size_t>(f.row[tt][m]) * a.K + k, v[j]);
                         else
 #pragma unroll
@@ -178,9 +178,9 @@ __global__ void __launch_bounds__(THREADS, 2) mx_small_kernel(const __grid_const
                     uint8_t* img = smem + off_b + st * B_STAGE;
                     uint8_t* sf = smem + off_sfb + st * SF_TILE;
 #pragma unroll
-                    for (int j = 0; j < TOK / 2; ++j) {
-                        if (2 * j >= n) break;
-                        const int m = 2 * j + half;
+                    for (int j = 0; j < TOK / 4; ++j) {
+                        const int m = m0 + 2 * j;
+                        if (m - (lane >> 4) >= n) break;
                         uint32_t sc;
                         const uint2 q = mxfp8_block8(v[j], lane, sc);
                         if (m < n) {
