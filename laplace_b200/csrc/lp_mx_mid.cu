@@ -21,7 +21,7 @@ using namespace tc;
 
 constexpr int THREADS = 384;
 constexpr int DRAIN_WARPS = 8;                 // two per quadrant of TMEM lanes
-constexpr int MAX_C = 8, MAX_STAGES = 10;
+constexpr int MAX_STAGES = 10;
 constexpr int A_STAGE = 128 * 128;             // 128 rows x 128 values, a byte each after the copy
 constexpr uint32_t SF_COL = 256;               // TMEM columns of the scales, behind two accumulators: two sets of 8
 constexpr size_t SMEM = 227 * 1024;
@@ -269,14 +269,16 @@ int clusters_of(int i) {
 // tiles: of a grouped call as many as there would be with an even-handed router
 template <int NT, bool GROUPED>
 int launch_nt(const CUtensorMap& map, const MxArgs& a, long long tiles, cudaStream_t st) {
-    // k over C CTAs: as few steps one after the other as can be, an exchange counted as EXCHANGE steps a tile
-    constexpr int EXCHANGE = 3;
+    // k over C CTAs: as few steps one after the other as can be, an exchange counted in steps by the tokens that it moves and the CTAs that meet.
+    // Measured, us with C = 1 / 2 / 4 / 8: 24 x 4096 x 4096 12.6 / 10.2 / 8.7 / 12.8, 24 x 14336 x 4096 31.9 / 19.5 / 13.7 / 17.6, 24 x 4096 x 14336
+    // 12.9 / 14.7 / 18.2 / 28.2, 48 x 4096 x 1024 11.8 / 9.9 / 8.1 / 7.3, 77 x 2816 x 8448 10.6 / 11.5 / 13.5 / 24.2, 128 x 4096 x 4096 13.4 / 13.7 / 11.6 / 20.7.
+    const int tokens = GROUPED ? NT / 2 : a.M;
     int best = 0;
     long long least = 1ll << 62;
     for (int i = 0; i < 4; ++i) {
         const int c = 1 << i, n = clusters_of<NT, GROUPED>(i);
         if (!n || a.kts < c) continue;
-        const long long steps = (tiles + n - 1) / n * ((a.kts + c - 1) / c + (c > 1 ? EXCHANGE : 0));
+        const long long steps = (tiles + n - 1) / n * ((a.kts + c - 1) / c + (c > 1 ? 2 + tokens / 9 + c / 2 : 0));
         if (steps < least) { least = steps; best = i; }
     }
     const int C = 1 << best;

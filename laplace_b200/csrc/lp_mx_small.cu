@@ -309,15 +309,18 @@ int launch_c(const CUtensorMap& map, SmallArgs a, int tiles, cudaStream_t st) {
 
 template <bool GROUPED>
 int launch_small(const CUtensorMap& map, const SmallArgs& a, int tiles, cudaStream_t st) {
-    // k over C CTAs: as few steps one after the other as can be, and a cluster's exchange counted as two
+    // k over C CTAs, so that the time is least: rounds of tiles, each the steps of a CTA (200 ns, or more where so many CTAs are at work that memory is
+    // what they wait for: 470 with all of them) and an exchange. Measured, one row, us with C = 1 / 2 / 4 / 8: 4096 x 1024 8.6 / 5.5 / 4.1 / 3.6, 4096 x 4096
+    // 8.8 / 6.1 / 5.9 / 7.5, 4096 x 14336 9.8 / 10.6 / 11.1 / 14.4, 14336 x 4096 25.5 / 14.7 / 9.8 / 12.6, eight experts 2048 x 1536 6.7 / 7.7 / 7.9 / 6.6.
     const int n[4] = {clusters_of<1, GROUPED>(), clusters_of<2, GROUPED>(), clusters_of<4, GROUPED>(), clusters_of<8, GROUPED>()};
     int best = 0;
     long long least = 1ll << 62;
     for (int i = 0; i < 4; ++i) {
         const int c = 1 << i;
         if (!n[i] || a.kts < c || stages_of(c, a.M) < QUANT) continue;
-        const long long steps = static_cast<long long>((tiles + n[i] - 1) / n[i]) * ((a.kts + c - 1) / c) + (c > 1 ? 2 : 0);
-        if (steps < least) { least = steps; best = i; }
+        const long long active = static_cast<long long>(tiles < n[i] ? tiles : n[i]) * c, step = active * 470 / (2 * ctx().sm_count);
+        const long long ns = (tiles + n[i] - 1) / n[i] * ((a.kts + c - 1) / c * (step > 200 ? step : 200) + (c > 1 ? 900 + 100 * c : 0));
+        if (ns < least) { least = ns; best = i; }
     }
     switch (best) {
         case 0: return launch_c<1, GROUPED>(map, a, tiles, st);
