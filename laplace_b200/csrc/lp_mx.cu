@@ -36,34 +36,39 @@ __global__ void __launch_bounds__(256) mxfp4_quantize_kernel(const T* __restrict
     const int part = threadIdx.x & 3;
     const long long b0 = static_cast<long long>(blockIdx.x) * QB;
     const int here = n_blocks - b0 < QB ? static_cast<int>(n_blocks - b0) : QB;
-    float v[QROUNDS][8] = {};
+    Eight<T> in[QROUNDS];
 #pragma unroll
     for (int i = 0; i < QROUNDS; ++i) {
         const int blk = (threadIdx.x >> 2) + 64 * i;
-        if (blk < here) load8(x + (b0 + blk) * 32 + part * 8, v[i]);
+        if (blk < here) in[i].load(x + (b0 + blk) * 32 + part * 8);
+        else in[i].zero();
     }
 #pragma unroll
     for (int i = 0; i < QROUNDS; ++i) {
         const int blk = (threadIdx.x >> 2) + 64 * i;
-        float a = amax8(v[i]);
-        a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 1));
-        a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 2));
-        const bool bad = !(a < __uint_as_float(0x7f800000u));            // infinity or NaN: the block stands for NaN
-        int s = static_cast<int>(__float_as_uint(a) >> 23) - 129;         // floor(log2(a)) - 2; 0 and numbers below the normal ones: the lowest
-        if (s < -127) s = -127;
+        uint32_t a = in[i].amax();
+        a = max(a, __shfl_xor_sync(0xffffffffu, a, 1));
+        a = max(a, __shfl_xor_sync(0xffffffffu, a, 2));
+        const bool bad = a >= 0x7f800000u;                                // infinity or NaN: the block stands for NaN
+        const int s = max(static_cast<int>(a >> 23) - 129, -127);         // floor(log2(a)) - 2; 0 and numbers below the normal ones: the lowest
         const float inv = pow2(-s);
-        uint32_t c = 0;                                                   // eight codes, value i in bits 4 i
-        if (!bad) {
+        float v[8];
+        in[i].values(v);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) c |= e2m1x2(v[i][2 * k] * inv, v[i][2 * k + 1] * inv) << (8 * k);
-        }
+        for (int k = 0; k < 8; ++k) v[k] *= inv;
+        const uint32_t c = bad ? 0 : e2m1x8(v);                           // eight codes, value i in bits 4 i
         const uint32_t o = __shfl_xor_sync(0xffffffffu, c, 2);            // lanes 0 and 1 hold values 0..15, lanes 2 and 3 16..31
-        // bytes 8 (part & 1) + 4 (part >> 1) .. + 3 of the sixteen
+        // bytes 8 (part & 1) + 4 (part >> 1) .. + 3 of the sixteen: four codes of c and o each, spread over bytes
         const int h = part >> 1;
-        const uint32_t lo = (h ? o : c) >> (16 * h), hi = (h ? c : o) >> (16 * h);
+        uint32_t lo = __byte_perm(c, o, h ? 0x4476 : 0x4410), hi = __byte_perm(c, o, h ? 0x4432 : 0x4454);
+        lo = (lo & 0xffu) | ((lo & 0xff00u) << 8);
+        hi = (hi & 0xffu) | ((hi & 0xff00u) << 8);
+        lo = (lo | (lo << 4)) & 0x0f0f0f0fu;
+        hi = (hi | (hi << 4)) & 0x0f0f0f0fu;
+        const uint32_t bytes = lo | (hi << 4);
         uint8_t* d = out + blk * 17 + 1 + (part & 1) * 8 + h * 4;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) d[k] = static_cast<uint8_t>(((lo >> (4 * k)) & 15u) | (((hi >> (4 * k)) & 15u) << 4));
+        for (int k = 0; k < 4; ++k) d[k] = static_cast<uint8_t>(bytes >> (8 * k));
         if (part == 0) out[blk * 17] = static_cast<uint8_t>(bad ? 255 : s + 127);
     }
     __syncthreads();

@@ -63,10 +63,12 @@ struct MxArgs {
 };
 #ifdef __CUDACC__
 
-// two values as e2m1, the first in the low four bits: to nearest, ties to even, magnitudes over 6 become 6
-__device__ __forceinline__ uint32_t e2m1x2(float a, float b) {
+// eight values as e2m1, the first in the lowest four bits: to nearest, ties to even, magnitudes over 6 become 6
+__device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
     uint32_t r;
-    asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n\tcvt.u32.u8 %0, t;\n\t}" : "=r"(r) : "f"(a), "f"(b));
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tcvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\tmov.b32 %0, {a, b, c, d};\n\t}"
+        : "=r"(r) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
     return r;
 }
 // the values of two e2m1 codes
@@ -82,25 +84,56 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(hi) : "f"(c), "f"(d));
     return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
 }
-template <class T> __device__ __forceinline__ void load8(const T* p, float (&v)[8]);
-template <> __device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-template <> __device__ __forceinline__ void load8<__half>(const __half* p, float (&v)[8]) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+// Eight values as they lie in memory; their fp32 values; the bits, as fp32, of their largest magnitude (infinity and NaN at or above 0x7f800000).
+template <class T> struct Eight;
+template <> struct Eight<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float* p) { a = __ldg(reinterpret_cast<const float4*>(p)); b = __ldg(reinterpret_cast<const float4*>(p) + 1); }
+    __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+    __device__ __forceinline__ void values(float (&v)[8]) const { v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w; }
+    __device__ __forceinline__ uint32_t amax() const {
+        float v[8];
+        values(v);
+        uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        v[2 * i] = f.x; v[2 * i + 1] = f.y;
+        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+        return m;
     }
+};
+// two 16-bit values a word: magnitudes compare as unsigned halves
+__device__ __forceinline__ uint32_t amax16(const uint4& w) {
+    const uint32_t m = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
+    return max(m & 0xffffu, m >> 16);
 }
-template <> __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&v)[8]) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+template <> struct Eight<__half> {
+    uint4 w;
+    __device__ __forceinline__ void load(const __half* p) { w = __ldg(reinterpret_cast<const uint4*>(p)); }
+    __device__ __forceinline__ void zero() { w = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ void values(float (&v)[8]) const {
+        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x[i]));
+            v[2 * i] = f.x; v[2 * i + 1] = f.y;
+        }
+    }
+    __device__ __forceinline__ uint32_t amax() const { return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(amax16(w))))) & 0x7fffffffu; }
+};
+template <> struct Eight<__nv_bfloat16> {
+    uint4 w;
+    __device__ __forceinline__ void load(const __nv_bfloat16* p) { w = __ldg(reinterpret_cast<const uint4*>(p)); }
+    __device__ __forceinline__ void zero() { w = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ void values(float (&v)[8]) const {
+        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(x[i] << 16); v[2 * i + 1] = __uint_as_float(x[i] & 0xffff0000u); }
+    }
+    __device__ __forceinline__ uint32_t amax() const { return amax16(w) << 16; }
+};
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+    Eight<float> e;
+    e.load(p);
+    e.values(v);
 }
 __device__ __forceinline__ float amax8(const float (&v)[8]) {
     float a = fabsf(v[0]);
