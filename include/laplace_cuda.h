@@ -265,8 +265,8 @@ int laplace_cuda_lm_head_dev(const float* x, const uint8_t* w, uint32_t type, fl
  * laplace_cuda_mxfp4_packed_size / _pack_dev: n_experts matrices of N rows of K values (one after the other; w at any
  *   alignment; one matrix: n_experts = 1) -> the packed layout, 128-byte aligned, 0.53 bytes per value and row tiles of 128.
  * laplace_cuda_mxfp4_gemm_dev: y[m][j] = sum_k xq[m][k] * w[j][k], where xq holds x as MXFP8: e4m3 values and, per 32 of them,
- *   the smallest power of two that keeps the largest magnitude within 448 times it, rounded to nearest even. Sums in fp32. A
- *   block of x with an infinity or a NaN makes its row of y NaN, as a NaN block of the weights makes its column. M = 0 is a call without effect.
+ *   the smallest power of two that keeps the largest magnitude within 448 times it, rounded to nearest even. Sums in fp32 (a
+ *   partial sum that leaves its range is infinite, whatever follows). A block of x with an infinity or a NaN makes its row of y NaN, as a NaN block of the weights makes its column. M = 0 is a call without effect.
  * laplace_cuda_mxfp4_moe_grouped_dev: the same for (token, expert) pairs, as laplace_cuda_moe_grouped_dev:
  *   y[p][j] = sum_k xq[pair_row[p]][k] * w[pair_expert[p]][j][k]; pair_row = NULL: pair p reads row p. Pairs in any order. A
  *   negative expert leaves its row of y untouched; an expert >= n_experts_total or a row outside [0, x_rows) does too and
@@ -402,7 +402,8 @@ int laplace_cuda_last_path(void);
 /* Which kernel the last matmul launched ran on: 1 = dp4a streaming, 2 = int8 MMA for a handful of rows and for experts
  * (mma.sync), 3 = int8 MMA tiles, 4 = tcgen05, 5 = tcgen05 with weights in two pieces, 6 = fp32 activations. For tests. */
 int laplace_cuda_last_kernel(void);
-/* How many CTAs worked on one tile of it together: 2 = a pair of SMs (tcgen05 cta_group::2), else 1. For tests. */
+/* How many CTAs worked on one tile of it together: 2 = a pair of SMs (tcgen05 cta_group::2), else 1. For tests. The
+ * laplace_cuda_mxfp4_* calls leave these three as they were. */
 int laplace_cuda_last_cta_group(void);
 /* Kernel launches issued by this library since the counter was last reset. */
 long long laplace_cuda_launch_count(int reset);

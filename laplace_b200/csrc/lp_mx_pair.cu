@@ -11,6 +11,9 @@
 //
 // Roles by warp: 0 copies, 1 MMA issue in the even CTA (owns the TMEM), word of the filled stages in the odd one, 4-11 drain (lane =
 // weight row). All waits are bounded; a wait that gives up raises the status word and the roles leave their loops.
+//
+// 2048 x 14336 x 4096: 540 cycles a step (512 are the tensor core's), 240 Gop in 75 to 87 us under the card's power limit (1.5 GHz), 108 with the quantizer; one
+// CTA with 128 x 256 took 610 cycles a step. 512 x 4096 x 14336 31.8 us, 512 x 4096 x 4096 17.3.
 #include "lp_mx.cuh"
 #include "lp_mx_mma.cuh"
 #include "lp_tc.cuh"

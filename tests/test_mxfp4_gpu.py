@@ -194,6 +194,24 @@ def test_zeros_and_extreme_scales():
     assert (np.abs(y.cpu().numpy() - want) <= ref.tolerance(K, mass)).all() and not y[1].any()
 
 
+@pytest.mark.parametrize("M", [1, 20, 200])
+def test_scales_from_end_to_end_of_their_range(M):
+    """Scales far from 1 on one side and as far the other way on the other: results are ordinary numbers, or so small that fp32 holds them with
+    fewer bits (there a step may be off by the smallest number that it holds)."""
+    from laplace_b200 import device
+    K, N = 64, 130
+    rng = np.random.default_rng(942)
+    for we, xe in ((0, 100), (1, 120), (20, 100), (60, 40), (127, -126), (200, -60), (250, -130), (20, -40)):
+        w = np.zeros((N, K // 32, 17), dtype=np.uint8)
+        w[..., 0] = we
+        w[..., 1:] = rng.integers(0, 256, (N, K // 32, 16))
+        x = (rng.standard_normal((M, K)) * 2.0 ** xe).astype(np.float32)
+        y = device.mxfp4_gemm(_dev(x), device.mxfp4_pack(_dev(w.reshape(-1)), N, K), M, K, N)
+        device.sync()
+        want, mass = ref.product(x, ref.dequantize_mxfp4(w).reshape(N, K))
+        assert (np.abs(y.cpu().numpy() - want) <= ref.tolerance(K, mass) + (K / 32 + 32) * 2.0 ** -149).all(), (we, xe)
+
+
 def test_rows_behind_the_last_stay():
     import torch
     from laplace_b200 import device
