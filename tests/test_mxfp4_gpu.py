@@ -244,7 +244,7 @@ def _routing(seed, T, E, k, skew):
 
 @pytest.mark.parametrize("T,E,k,K,N,skew", [(1, 32, 8, 2048, 384, 0.), (1, 4, 1, 32, 1, 0.), (4, 32, 8, 352, 300, 3.), (5, 4, 2, 160, 200, 1.), (24, 60, 4, 768, 130, 1.), (100, 8, 3, 256, 520, 2.),
                                             (256, 32, 8, 512, 256, 1.5), (600, 4, 2, 96, 257, 1.), (700, 128, 8, 128, 96, 2.), (40, 1, 1, 288, 300, 0.), (1400, 3, 2, 1056, 700, 1.),
-                                            (3000, 8, 2, 96, 130, 2.), (20000, 4, 1, 32, 40, 1.), (2000, 1500, 3, 64, 24, 2.), (700, 600, 3, 32, 33, 3.), (60000, 3, 1, 32, 8, 1.)])
+                                            (3000, 8, 2, 96, 130, 2.), (32, 1, 1, 288, 300, 0.), (31, 2, 1, 96, 140, 3.), (33, 1, 1, 64, 64, 0.), (20000, 4, 1, 32, 40, 1.), (2000, 1500, 3, 64, 24, 2.), (700, 600, 3, 32, 33, 3.), (60000, 3, 1, 32, 8, 1.)])
 @pytest.mark.parametrize("form", ["shared", "own", "elsewhere"])
 def test_grouped(T, E, k, K, N, skew, form):
     from laplace_b200 import device
@@ -297,6 +297,44 @@ def test_grouped_bad_indices_are_skipped_and_reported():
             if p != bad:
                 want, mass = ref.product(x[row[p]:row[p] + 1], v.reshape(E, N, K)[expert[p]])
                 _close(y[p:p + 1], want, mass, K)
+
+
+# ---- large ones ---------------------------------------------------------------------------------------------------------------
+
+def test_results_behind_the_32_bit_range():
+    """More than 2^31 results: rows from everywhere are right."""
+    import torch
+    from laplace_b200 import device
+    M, K, N = 140001, 64, 16400
+    w, v = _blocks(1400, N, K)
+    g = torch.Generator(device="cuda").manual_seed(1401)
+    x = torch.randn(M, K, device="cuda", generator=g)
+    y = device.mxfp4_gemm(x, device.mxfp4_pack(_dev(w), N, K), M, K, N)
+    device.sync()
+    for m in (0, 1, 65535, 130943, 130944, 131072, M - 1):
+        _close(y[m:m + 1], *ref.product(x[m:m + 1].cpu().numpy(), v), K, f"row {m}")
+
+
+def test_weights_behind_the_32_bit_range():
+    """Experts of more than 2^32 packed bytes: the first and the last are right, for a few pairs, for many, and as one matrix's rows."""
+    import torch
+    from laplace_b200 import device
+    E, K, N = 66, 8192, 16384
+    g = torch.Generator(device="cuda").manual_seed(1410)
+    w = torch.randint(0, 256, (E * N * (K // 32), 17), dtype=torch.uint8, device="cuda", generator=g)
+    w[:, 0] = w[:, 0] % 8 + 116
+    packed = device.mxfp4_pack(w.view(-1), N, K, E)
+    assert packed.numel() > 1 << 32
+    per = N * (K // 32)
+    values = {e: ref.dequantize_mxfp4(w[e * per:e * per + 64 * (K // 32)].cpu().numpy()).reshape(64, K) for e in (0, E - 1)}      # of the expert's first 64 rows
+    del w
+    for T in (3, 200, 1000):
+        x = _act(1411, T, K)
+        expert = np.where(np.arange(T) % 3 == 0, 0, E - 1).astype(np.int32)
+        y = device.mxfp4_moe_grouped(_dev(x), packed, _dev(expert), None, E, K, N)
+        device.sync()
+        for p in (0, 1, T - 1):
+            _close(y[p:p + 1, :64], *ref.product(x[p:p + 1], values[int(expert[p])]), K, f"{T} pairs, pair {p}")
 
 
 # ---- streams, graphs, timing ----------------------------------------------------------------------------------------------
