@@ -191,6 +191,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx_mid_kernel(const __grid_constan
             // Owner o has tokens o * run .. of the tile; its buffer is [CTA of the cluster][token / 4][row][4 tokens].
             const int run = ((s.n + C - 1) / C + 3) & ~3;
             const uint32_t part = static_cast<uint32_t>(run) * 512;
+            const float per_run = 1.0f / static_cast<float>(run);
             if (i && !wait_pair(bar(f.avail), (i - 1) & 1, abort_flag, a.err, DEV_TIMEOUT_DRAIN)) break;
             __syncwarp();
 #pragma unroll
@@ -199,7 +200,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx_mid_kernel(const __grid_constan
                 for (int k = 0; k < 32; k += 4) {
                     const int c = 32 * half + 64 * j + k;
                     if (c >= s.n) break;
-                    const int o = c / run;
+                    const int o = static_cast<int>((static_cast<float>(c) + 0.5f) * per_run);       // c / run: half a token from either border at least, c < 128
                     st_cluster4(map_to_rank(sb + off_recv + rank * part + ((c - o * run) * 128 + r * 4) * 4, o), v[j][k], v[j][k + 1], v[j][k + 2], v[j][k + 3]);
                 }
             __syncwarp();
