@@ -10,7 +10,7 @@
 // into shared memory takes 7.5. 2,048 pairs of 128 experts 2048 x 1536 (214 MB) 43 us, 4.9 TB/s, 48 with grouping and quantizer.
 //
 // Roles by warp: 0 copies, 1 MMA issue (owns the TMEM), 4-11 drain (lane = weight row), sums and output. All waits are bounded; a wait that
-// gives up raises the status word and the roles leave their loops. No CTA leaves before its cluster is done.
+// gives up raises the status word and the roles leave their loops.
 #include "lp_mx.cuh"
 #include "lp_mx_mma.cuh"
 #include "lp_tc.cuh"
@@ -208,20 +208,28 @@ __global__ void __launch_bounds__(THREADS, 1) mx_mid_kernel(const __grid_constan
             if (!wait_pair(bar(f.recv), i & 1, abort_flag, a.err, DEV_TIMEOUT_DRAIN)) break;
             __syncwarp();
             const int m0 = rank * run, mine = min(run, s.n - m0);
-            for (int g = half; 4 * g < mine; g += 2) {
-                const float4* p = reinterpret_cast<const float4*>(smem + off_recv) + g * 128 + r;
-                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+            for (int g0 = half; 4 * g0 < mine; g0 += 8) {      // four groups of four tokens at a time
+                const float4* p = reinterpret_cast<const float4*>(smem + off_recv) + g0 * 128 + r;
+                float4 sum[4] = {};
+#pragma unroll 1
                 for (int c = 0; c < C; ++c) {
-                    const float4 o = p[c * (run / 4) * 128];
-                    sum.x += o.x; sum.y += o.y; sum.z += o.z; sum.w += o.w;
-                }
-                const float e[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if (4 * g + k >= mine) break;
-                    const int m = m0 + 4 * g + k, to = GROUPED ? __ldg(a.out_row + s.row0 + m) : m;
-                    if (to >= 0 && col < a.N) a.y[static_cast<size_t>(to) * a.N + col] = e[k];
+                    for (int u = 0; u < 4; ++u) {
+                        if (4 * (g0 + 2 * u) >= mine) break;
+                        const float4 o = p[(c * (run / 4) + 2 * u) * 128];
+                        sum[u].x += o.x; sum[u].y += o.y; sum[u].z += o.z; sum[u].w += o.w;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    if (4 * (g0 + 2 * u) >= mine) break;
+                    const float e[4] = {sum[u].x, sum[u].y, sum[u].z, sum[u].w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int at = 4 * (g0 + 2 * u) + k, m = m0 + at;
+                        const int to = !GROUPED || at >= mine ? m : __ldg(a.out_row + s.row0 + m);
+                        store_if(at < mine && to >= 0 && col < a.N, a.y + static_cast<size_t>(to) * a.N + col, e[k]);
+                    }
                 }
             }
             if (t + clusters < tiles) {             // there is a next tile: the buffer is free for every CTA
@@ -234,8 +242,10 @@ __global__ void __launch_bounds__(THREADS, 1) mx_mid_kernel(const __grid_constan
     }
     __syncwarp();
     fence_before();
-    if (C > 1) { cluster_arrive(); cluster_wait(); }
-    else __syncthreads();
+    __syncthreads();
+    // What the others send here has been waited for, and who this CTA sends to waits for that: it may go. After a wait that gave up it does not until
+    // every CTA of the cluster is here or gone.
+    if (C > 1 && *abort_flag) { cluster_arrive(); cluster_wait(); }
     if (warp == 1) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");

@@ -12,7 +12,7 @@
 //
 // A cluster of C CTAs takes tiles (128 weight rows x up to 8 tokens) number cluster, cluster + clusters, ...; the i-th of them is owned by CTA i % C.
 // Roles by warp: 0 copies, 1 MMA issue (owns the TMEM), 2, 3, 8-13 quantizers (in pairs, four rows each), 4-7 drain (lane = weight row), sums and output. All waits are
-// bounded; a wait that gives up raises the status word and the roles leave their loops. No CTA leaves before its cluster is done.
+// bounded; a wait that gives up raises the status word and the roles leave their loops.
 #include "lp_mx.cuh"
 #include "lp_mx_mma.cuh"
 #include "lp_tc.cuh"
@@ -256,8 +256,10 @@ __global__ void __launch_bounds__(THREADS, 2) mx_small_kernel(const __grid_const
     }
     __syncwarp();
     fence_before();
-    if (C > 1) { cluster_arrive(); cluster_wait(); }
-    else __syncthreads();
+    __syncthreads();
+    // What the others send here has been waited for, and who this CTA sends to waits for that: it may go. After a wait that gave up it does not until
+    // every CTA of the cluster is here or gone.
+    if (C > 1 && *abort_flag) { cluster_arrive(); cluster_wait(); }
     if (warp == 1) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(TMEM_COLS) : "memory");
