@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(GROUP_THREADS) mx_count_kernel(const int* __re
     }
 }
 constexpr int COUNT_FROM = 4097;
-__global__ void __launch_bounds__(GROUP_THREADS) mx_group_kernel(const int* __restrict__ pair_expert, int P, int E, int tile_w, int tile_groups,
+__global__ void __launch_bounds__(GROUP_THREADS) mx_group_kernel(const int* __restrict__ pair_expert, int P, int E, int tile_log2, int tile_groups,
                                                                  const int* __restrict__ counts, int2* __restrict__ place, int* __restrict__ out_row, int4* __restrict__ tab,
                                                                  int4* __restrict__ work, int row_tiles, int kts, int n, int* err) {
     constexpr int U = 16;
@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(GROUP_THREADS) mx_group_kernel(const int* __re
     int rows = 0, tiles = 0;               // of the experts before
     for (int e0 = 0; e0 < E; e0 += threads) {
         const int e = e0 + threadIdx.x, c = e < E ? count[e] : 0;
-        const int r = (c + 7) & ~7, t = (c + tile_w - 1) / tile_w;
+        const int r = (c + 7) & ~7, t = (c + (1 << tile_log2) - 1) >> tile_log2;
         int ri = r, ti = t;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -341,13 +341,14 @@ __global__ void __launch_bounds__(GROUP_THREADS) mx_group_kernel(const int* __re
                 const unsigned all = __ballot_sync(0xffffffffu, x[i] == e);
                 if (x[i] == e) {
                     const int r = at + __popc(all & ((1u << lane) - 1)), p = q + 32 * i + lane;
-                    place[p] = make_int2(s + r, (t0 + r / tile_w) * tile_groups * 128 + r % tile_w);
+                    place[p] = make_int2(s + r, (t0 + (r >> tile_log2)) * tile_groups * 128 + (r & ((1 << tile_log2) - 1)));
                     out_row[s + r] = p;
                 }
                 at += __popc(all);
             }
         }
-        for (int i = threadIdx.x; i * tile_w < c; i += threads) tab[t0 + i] = make_int4(e, s + i * tile_w, min(tile_w, c - i * tile_w), (t0 + i) * tile_groups);
+        for (int i = threadIdx.x; i << tile_log2 < c; i += threads)
+            tab[t0 + i] = make_int4(e, s + (i << tile_log2), min(1 << tile_log2, c - (i << tile_log2)), (t0 + i) * tile_groups);
     }
 }
 // threads of the grouping block: the instructions of all its warps are what the launch waits for (2,048 pairs: 1024 threads 8.7 us, 256 6.4)
@@ -451,7 +452,7 @@ int launch_product(const float* x, int x_rows, const uint8_t* packed, const int*
             c.launches++;
             if (rc) return rc;
         }
-        rc = launch_early(mx_group_kernel, grid, group_threads(rows), 3 * static_cast<size_t>(experts) * sizeof(int), st, pair_expert, rows, experts, p.tile_w, p.tile_groups,
+        rc = launch_early(mx_group_kernel, grid, group_threads(rows), 3 * static_cast<size_t>(experts) * sizeof(int), st, pair_expert, rows, experts, __builtin_ctz(p.tile_w), p.tile_groups,
                           static_cast<const int*>(rows >= COUNT_FROM ? counts : nullptr), place, reinterpret_cast<int*>(ws + p.out_row), reinterpret_cast<int4*>(ws + p.tab),
                           reinterpret_cast<int4*>(ws + p.work), p.row_tiles, p.kts, units, c.d_err);
         c.launches++;
