@@ -41,18 +41,20 @@ template <int NT> constexpr int stages_of(int C) {
     return s < MAX_STAGES ? s : MAX_STAGES;
 }
 
-template <int NT, bool GROUPED>
-__global__ void __launch_bounds__(THREADS, 1) mx_mid_kernel(const __grid_constant__ CUtensorMap map, const MxArgs a, const int C, const int S) {
+// SPLIT: clusters of C > 1 CTAs. (A kernel of its own for C = 1: the code that either drags along is fetched by every SM of every launch, 0.4 us.)
+template <int NT, bool GROUPED, bool SPLIT>
+__global__ void __launch_bounds__(THREADS, 1) mx_mid_kernel(const __grid_constant__ CUtensorMap map, const MxArgs a, const int cluster_ctas, const int S) {
+    const int C = SPLIT ? cluster_ctas : 1;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t sb = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem = smem_raw + (sb - smem_u32(smem_raw));
     const uint32_t off_b = S * A_STAGE, off_sfa = off_b + S * NT * 128, off_sfb = off_sfa + S * SF_TILE, off_recv = off_sfb + S * SF_TILE,
-                   off_fixed = off_recv + (C == 1 ? 0 : (NT + 4 * C) * 512);
+                   off_fixed = off_recv + (SPLIT ? (NT + 4 * C) * 512 : 0);
     Fixed& f = *reinterpret_cast<Fixed*>(smem + off_fixed);
     volatile int* abort_flag = &f.abort;
     auto bar = [&](const uint64_t& b) { return smem_u32(&b); };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = C > 1 ? static_cast<int>(pair_rank()) : 0;
+    const int rank = SPLIT ? static_cast<int>(pair_rank()) : 0;
     if (threadIdx.x == 0) {
         for (int i = 0; i < S; ++i) { mbar_init(bar(f.full[i]), 1); mbar_init(bar(f.empty[i]), 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(bar(f.tfull[i]), 1); mbar_init(bar(f.tempty[i]), DRAIN_WARPS); }
@@ -69,7 +71,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx_mid_kernel(const __grid_constan
     fence_before();
     __syncthreads();
     fence_after();
-    if (C > 1) cluster_arrive();                   // barriers are there for the other CTAs; waited for where they are used first
+    if (SPLIT) cluster_arrive();                   // barriers are there for the other CTAs; waited for where they are used first
     const uint32_t tmem = f.tmem;
     // Experts: the table of token tiles is made by the kernels before this one. One matrix: the weights may be copied meanwhile; the quantizer
     // before this kernel lets it start only after it has itself waited for what is before it in the stream, weights' writers included.
@@ -118,7 +120,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx_mid_kernel(const __grid_constan
         }
         if (!ok)                                    // what is in flight lands before the CTA goes
             for (int i = 0; i < 1000; ++i) __nanosleep(1000);
-        if (C > 1) cluster_wait();
+        if (SPLIT) cluster_wait();
     } else if (warp == 1 && elect_one()) {
         int st = 0, parity = 0, i = 0, set = 0;      // set: of TMEM columns for the scales
         bool ok = true;
@@ -141,12 +143,12 @@ __global__ void __launch_bounds__(THREADS, 1) mx_mid_kernel(const __grid_constan
             }
             if (ok) commit(bar(f.tfull[acc]));
         }
-        if (C > 1) cluster_wait();
+        if (SPLIT) cluster_wait();
     } else if (warp >= 4) {
         const int id = threadIdx.x - 128, half = id >> 7, r = id & 127;      // r: weight row of the tile
         const uint32_t quadrant = static_cast<uint32_t>(warp & 3) * 32u << 16;
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-        if (C > 1) cluster_wait();
+        if (SPLIT) cluster_wait();
         int i = 0;
         for (int t = cluster; t < tiles; t += clusters, ++i) {
             const int acc = i & 1;
@@ -165,7 +167,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx_mid_kernel(const __grid_constan
             fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(f.tempty[acc]));
-            if (C == 1) {
+            if constexpr (!SPLIT) {
 #pragma unroll
                 for (int j = 0; j < J; ++j) {
                     const int c0 = 32 * half + 64 * j, here = min(32, s.n - c0);
@@ -186,58 +188,58 @@ __global__ void __launch_bounds__(THREADS, 1) mx_mid_kernel(const __grid_constan
                     }
                     __syncwarp();
                 }
-                continue;
-            }
-            // Owner o has tokens o * run .. of the tile; its buffer is [CTA of the cluster][token / 4][row][4 tokens].
-            const int run = ((s.n + C - 1) / C + 3) & ~3;
-            const uint32_t part = static_cast<uint32_t>(run) * 512;
-            const float per_run = 1.0f / static_cast<float>(run);
-            if (i && !wait_pair(bar(f.avail), (i - 1) & 1, abort_flag, a.err, DEV_TIMEOUT_DRAIN)) break;
-            __syncwarp();
+            } else {
+                // Owner o has tokens o * run .. of the tile; its buffer is [CTA of the cluster][token / 4][row][4 tokens].
+                const int run = ((s.n + C - 1) / C + 3) & ~3;
+                const uint32_t part = static_cast<uint32_t>(run) * 512;
+                const float per_run = 1.0f / static_cast<float>(run);
+                if (i && !wait_pair(bar(f.avail), (i - 1) & 1, abort_flag, a.err, DEV_TIMEOUT_DRAIN)) break;
+                __syncwarp();
 #pragma unroll
-            for (int j = 0; j < J; ++j)
+                for (int j = 0; j < J; ++j)
 #pragma unroll
-                for (int k = 0; k < 32; k += 4) {
-                    const int c = 32 * half + 64 * j + k;
-                    if (c >= s.n) break;
-                    const int o = static_cast<int>((static_cast<float>(c) + 0.5f) * per_run);       // c / run: half a token from either border at least, c < 128
-                    st_cluster4(map_to_rank(sb + off_recv + rank * part + ((c - o * run) * 128 + r * 4) * 4, o), v[j][k], v[j][k + 1], v[j][k + 2], v[j][k + 3]);
-                }
-            __syncwarp();
-            if (lane < C) arrive_release(map_to_rank(bar(f.recv), lane));
-            if (!wait_pair(bar(f.recv), i & 1, abort_flag, a.err, DEV_TIMEOUT_DRAIN)) break;
-            __syncwarp();
-            const int m0 = rank * run, mine = min(run, s.n - m0);
-            for (int g0 = half; 4 * g0 < mine; g0 += 8) {      // four groups of four tokens at a time
-                const float4* p = reinterpret_cast<const float4*>(smem + off_recv) + g0 * 128 + r;
-                float4 sum[4] = {};
+                    for (int k = 0; k < 32; k += 4) {
+                        const int c = 32 * half + 64 * j + k;
+                        if (c >= s.n) break;
+                        const int o = static_cast<int>((static_cast<float>(c) + 0.5f) * per_run);       // c / run: half a token from either border at least, c < 128
+                        st_cluster4(map_to_rank(sb + off_recv + rank * part + ((c - o * run) * 128 + r * 4) * 4, o), v[j][k], v[j][k + 1], v[j][k + 2], v[j][k + 3]);
+                    }
+                __syncwarp();
+                if (lane < C) arrive_release(map_to_rank(bar(f.recv), lane));
+                if (!wait_pair(bar(f.recv), i & 1, abort_flag, a.err, DEV_TIMEOUT_DRAIN)) break;
+                __syncwarp();
+                const int m0 = rank * run, mine = min(run, s.n - m0);
+                for (int g0 = half; 4 * g0 < mine; g0 += 8) {      // four groups of four tokens at a time
+                    const float4* p = reinterpret_cast<const float4*>(smem + off_recv) + g0 * 128 + r;
+                    float4 sum[4] = {};
 #pragma unroll 1
-                for (int c = 0; c < C; ++c) {
+                    for (int c = 0; c < C; ++c) {
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            if (4 * (g0 + 2 * u) >= mine) break;
+                            const float4 o = p[(c * (run / 4) + 2 * u) * 128];
+                            sum[u].x += o.x; sum[u].y += o.y; sum[u].z += o.z; sum[u].w += o.w;
+                        }
+                    }
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
                         if (4 * (g0 + 2 * u) >= mine) break;
-                        const float4 o = p[(c * (run / 4) + 2 * u) * 128];
-                        sum[u].x += o.x; sum[u].y += o.y; sum[u].z += o.z; sum[u].w += o.w;
+                        const float e[4] = {sum[u].x, sum[u].y, sum[u].z, sum[u].w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int at = 4 * (g0 + 2 * u) + k, m = m0 + at;
+                            const int to = !GROUPED || at >= mine ? m : __ldg(a.out_row + s.row0 + m);
+                            store_if(at < mine && to >= 0 && col < a.N, a.y + static_cast<size_t>(to) * a.N + col, e[k]);
+                        }
                     }
                 }
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    if (4 * (g0 + 2 * u) >= mine) break;
-                    const float e[4] = {sum[u].x, sum[u].y, sum[u].z, sum[u].w};
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int at = 4 * (g0 + 2 * u) + k, m = m0 + at;
-                        const int to = !GROUPED || at >= mine ? m : __ldg(a.out_row + s.row0 + m);
-                        store_if(at < mine && to >= 0 && col < a.N, a.y + static_cast<size_t>(to) * a.N + col, e[k]);
-                    }
+                if (t + clusters < tiles) {             // there is a next tile: the buffer is free for every CTA
+                    __syncwarp();
+                    if (lane < C) arrive_release(map_to_rank(bar(f.avail), lane));
                 }
-            }
-            if (t + clusters < tiles) {             // there is a next tile: the buffer is free for every CTA
-                __syncwarp();
-                if (lane < C) arrive_release(map_to_rank(bar(f.avail), lane));
             }
         }
-    } else if (C > 1) {
+    } else if (SPLIT) {
         cluster_wait();
     }
     __syncwarp();
@@ -245,7 +247,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx_mid_kernel(const __grid_constan
     __syncthreads();
     // What the others send here has been waited for, and who this CTA sends to waits for that: it may go. After a wait that gave up it does not until
     // every CTA of the cluster is here or gone.
-    if (C > 1 && *abort_flag) { cluster_arrive(); cluster_wait(); }
+    if (SPLIT && *abort_flag) { cluster_arrive(); cluster_wait(); }
     if (warp == 1) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
@@ -271,8 +273,9 @@ int clusters_of(int i) {
         cfg.gridDim = dim3(1 << i);
         cfg.numAttrs = 1;
         int got = 0;
-        const bool ok = cudaFuncSetAttribute(mx_mid_kernel<NT, GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) == cudaSuccess &&
-                        (i == 0 || cudaOccupancyMaxActiveClusters(&got, mx_mid_kernel<NT, GROUPED>, &cfg) == cudaSuccess);
+        const bool ok = cudaFuncSetAttribute(mx_mid_kernel<NT, GROUPED, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) == cudaSuccess &&
+                        cudaFuncSetAttribute(mx_mid_kernel<NT, GROUPED, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) == cudaSuccess &&
+                        (i == 0 || cudaOccupancyMaxActiveClusters(&got, mx_mid_kernel<NT, GROUPED, true>, &cfg) == cudaSuccess);
         n[i] = !ok ? 0 : i == 0 ? ctx().sm_count : got;
         cudaGetLastError();
     }
@@ -299,7 +302,8 @@ int launch_nt(const CUtensorMap& map, const MxArgs& a, long long tiles, cudaStre
     cudaLaunchConfig_t cfg = config(C, attr, st);
     cfg.gridDim = dim3(clusters_of<NT, GROUPED>(best) * C);
     ctx().launches++;
-    return cuda_check(cudaLaunchKernelEx(&cfg, mx_mid_kernel<NT, GROUPED>, map, a, C, stages_of<NT>(C)), "mx_mid launch");
+    return cuda_check(C > 1 ? cudaLaunchKernelEx(&cfg, mx_mid_kernel<NT, GROUPED, true>, map, a, C, stages_of<NT>(C))
+                            : cudaLaunchKernelEx(&cfg, mx_mid_kernel<NT, GROUPED, false>, map, a, C, stages_of<NT>(C)), "mx_mid launch");
 }
 
 }  // namespace
