@@ -390,7 +390,7 @@ Plan plan_of(int rows, int experts, int K, int N) {
     p.img_rows = static_cast<int>((most + 7) & ~7ll);
     const int per = experts ? (rows + experts - 1) / experts : rows;
     p.nt = per <= 32 ? 32 : per <= 64 ? 64 : per <= 128 ? 128 : 256;
-    const bool pairs = p.nt == 256;
+    bool pairs = p.nt == 256;
     p.row_tiles = pairs ? (p.rts + 1) / 2 : p.rts;
     p.tiles_m = (rows + p.nt - 1) / p.nt;
     p.tile_w = p.nt;
@@ -402,6 +402,14 @@ Plan plan_of(int rows, int experts, int K, int N) {
             const int w = round32((rows + m - 1) / m), tiles_m = (rows + w - 1) / w;
             const Shared s = share_out(tiles_m * p.row_tiles, w, p.kts, ctx().sm_count / 2);
             if (s.cycles < least) { least = s.cycles; p.tiles_m = tiles_m; p.tile_w = w; p.share = s.cut; }
+        }
+        // Or tiles of 128 rows x 128 tokens at the most on single SMs, whose launch and first copies take 4 us less (us, pairs / single SMs: 256 x 4096 x 4096
+        // 15.3 / 13.2, 512 x 4096 x 4096 17.4 / 14.9, 300 x 2816 x 1408 15.0 / 9.7; two rounds of tiles: 600 x 4096 x 4096 18.3 on pairs)
+        const int m = (rows + 127) / 128, w = ((rows + m - 1) / m + 7) & ~7, tiles_m = (rows + w - 1) / w;
+        if (mx_mid_ns(static_cast<long long>(tiles_m) * p.rts, p.kts, w) < least * 100 / 185 + 4000) {
+            pairs = false;
+            p.nt = 128; p.tile_w = w; p.tiles_m = tiles_m; p.row_tiles = p.rts;
+            p.share = Cut{tiles_m * p.rts, 0, 0};
         }
     }
     p.n_counters = pairs ? mx_pair_counters() : 0;
@@ -466,7 +474,7 @@ int launch_product(const float* x, int x_rows, const uint8_t* packed, const int*
     CUtensorMap map;
     if (!mx_weights_map(&map, a.q, static_cast<size_t>(GROUPED ? experts : 1) * p.rts * p.kts)) return LAPLACE_ERR_CUDA;
     if (p.nt == 256) return launch_mx_pair(map, a, GROUPED, st);
-    return launch_mx_mid(map, a, p.nt, static_cast<long long>(GROUPED ? (experts < rows ? experts : rows) : 1) * p.rts, GROUPED, st);
+    return launch_mx_mid(map, a, p.nt, GROUPED ? static_cast<long long>(experts < rows ? experts : rows) * p.rts : p.share.tiles, GROUPED, st);
 }
 
 // rows: token tiles times row tiles are counted in 32 bits

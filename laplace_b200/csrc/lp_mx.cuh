@@ -171,6 +171,7 @@ __device__ __forceinline__ uint2 mxfp8_block8(const float (&v)[8], int lane, uin
 size_t mx_pair_part_bytes();
 int    mx_pair_counters();
 int    launch_mx_pair(const CUtensorMap& map, const mx::MxArgs& a, bool grouped, cudaStream_t st);
+long long mx_mid_ns(long long tiles, int kts, int tokens);
 int    launch_mx_mid(const CUtensorMap& map, const mx::MxArgs& a, int nt, long long tiles, bool grouped, cudaStream_t st);
 bool   mx_small_takes(int rows, bool grouped);
 int    launch_mx_small(const float* x, int x_rows, const uint8_t* packed, const int* pair_expert, const int* pair_row, int rows, int experts, float* y, int K, int N, cudaStream_t st);

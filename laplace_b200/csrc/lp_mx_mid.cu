@@ -1,5 +1,5 @@
-// lp_mx_mid.cu - products of packed MXFP4 weights and quantized rows, tiles of 128 weight rows x up to 128 tokens: 9 to 128 rows of one matrix, or
-// experts with up to 128 pairs on average. Formats and layouts: lp_mx.cu, the instruction: lp_mx_mma.cuh.
+// lp_mx_mid.cu - products of packed MXFP4 weights and quantized rows, tiles of 128 weight rows x up to 128 tokens: 9 rows of one matrix and more, while its
+// tiles fit on the SMs at once, or experts with up to 128 pairs on average. Formats and layouts: lp_mx.cu, the instruction: lp_mx_mma.cuh.
 //
 // Bound by the weights' way from memory. A cluster of C CTAs takes tiles number cluster, cluster + clusters, ...; its CTAs share out k where there are
 // fewer tiles than SMs, and C is 1 where there are enough. A CTA sends its part of a tile's results into the shared memory of their owners
@@ -85,7 +85,8 @@ __global__ void __launch_bounds__(THREADS, 1) mx_mid_kernel(const __grid_constan
             const int4 e = __ldg(a.tab + t / a.rts);
             return Tile{e.x, t % a.rts, e.y, e.z, e.w};
         }
-        return Tile{0, t, 0, a.M, 0};              // one token tile
+        const int m = t % a.tiles_m, row0 = m * a.tile_w;
+        return Tile{0, t / a.tiles_m, row0, min(a.tile_w, a.M - row0), m};      // (up to 128 tokens: a group of scales each)
     };
 
     if (warp == 0 && elect_one()) {
@@ -181,7 +182,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx_mid_kernel(const __grid_constan
                             store_if(k < here && m >= 0 && col < a.N, a.y + static_cast<size_t>(m) * a.N + col, v[j][k]);
                         }
                     } else if (col < a.N) {
-                        float* q = a.y + static_cast<size_t>(c0) * a.N + col;
+                        float* q = a.y + static_cast<size_t>(s.row0 + c0) * a.N + col;
 #pragma unroll
                         for (int k = 0; k < 32; ++k)
                             if (k < here) q[static_cast<size_t>(k) * a.N] = v[j][k];
@@ -228,7 +229,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx_mid_kernel(const __grid_constan
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             const int at = 4 * (g0 + 2 * u) + k, m = m0 + at;
-                            const int to = !GROUPED || at >= mine ? m : __ldg(a.out_row + s.row0 + m);
+                            const int to = !GROUPED || at >= mine ? s.row0 + m : __ldg(a.out_row + s.row0 + m);
                             store_if(at < mine && to >= 0 && col < a.N, a.y + static_cast<size_t>(to) * a.N + col, e[k]);
                         }
                     }
@@ -282,21 +283,25 @@ int clusters_of(int i) {
     return n[i];
 }
 
-// tiles: of a grouped call as many as there would be with an even-handed router
+// k over C CTAs, so that the time is least: rounds of tiles, each the steps of a CTA and an exchange by the tokens that it moves and the CTAs that meet.
+// Measured, us with C = 1 / 2 / 4 / 8: 24 x 4096 x 4096 12.2 / 10.0 / 8.1 / 12.0, 24 x 14336 x 4096 31.7 / 19.4 / 13.7 / 17.0, 24 x 4096 x 14336
+// 13.0 / 14.3 / 17.4 / 27.3, 48 x 4096 x 1024 12.0 / 9.8 / 8.1 / 7.3, 77 x 2816 x 8448 10.6 / 11.1 / 13.3 / 23.7, 128 x 4096 x 4096 13.4 / 13.3 / 11.5 / 20.0.
+// tiles: of a grouped call as many as there would be with an even-handed router. Returns ns; best: log2 C.
 template <int NT, bool GROUPED>
-int launch_nt(const CUtensorMap& map, const MxArgs& a, long long tiles, cudaStream_t st) {
-    // k over C CTAs: as few steps one after the other as can be, an exchange counted in steps by the tokens that it moves and the CTAs that meet.
-    // Measured, us with C = 1 / 2 / 4 / 8: 24 x 4096 x 4096 12.6 / 10.2 / 8.7 / 12.8, 24 x 14336 x 4096 31.9 / 19.5 / 13.7 / 17.6, 24 x 4096 x 14336
-    // 12.9 / 14.7 / 18.2 / 28.2, 48 x 4096 x 1024 11.8 / 9.9 / 8.1 / 7.3, 77 x 2816 x 8448 10.6 / 11.5 / 13.5 / 24.2, 128 x 4096 x 4096 13.4 / 13.7 / 11.6 / 20.7.
-    const int tokens = GROUPED ? NT / 2 : a.M;
-    int best = 0;
+long long share_k(long long tiles, int kts, int tokens, int& best) {
     long long least = 1ll << 62;
     for (int i = 0; i < 4; ++i) {
         const int c = 1 << i, n = clusters_of<NT, GROUPED>(i);
-        if (!n || a.kts < c) continue;
-        const long long steps = (tiles + n - 1) / n * ((a.kts + c - 1) / c + (c > 1 ? 2 + tokens / 9 + c / 2 : 0));
-        if (steps < least) { least = steps; best = i; }
+        if (!n || kts < c) continue;
+        const long long ns = (tiles + n - 1) / n * ((kts + c - 1) / c * (230 + tokens / 2) + (c > 1 ? 240 * (2 + tokens / 9 + c / 2) : 0));
+        if (ns < least) { least = ns; best = i; }
     }
+    return least;
+}
+template <int NT, bool GROUPED>
+int launch_nt(const CUtensorMap& map, const MxArgs& a, long long tiles, cudaStream_t st) {
+    int best = 0;
+    share_k<NT, GROUPED>(tiles, a.kts, GROUPED ? NT / 2 : a.tile_w < a.M ? a.tile_w : a.M, best);
     const int C = 1 << best;
     cudaLaunchAttribute attr[2];
     cudaLaunchConfig_t cfg = config(C, attr, st);
@@ -307,6 +312,12 @@ int launch_nt(const CUtensorMap& map, const MxArgs& a, long long tiles, cudaStre
 }
 
 }  // namespace
+
+// Time of the tiles of one matrix, `tokens` (65 to 128) each, on this kernel.
+long long mx_mid_ns(long long tiles, int kts, int tokens) {
+    int best;
+    return share_k<128, false>(tiles, kts, tokens, best);
+}
 
 int launch_mx_mid(const CUtensorMap& map, const MxArgs& a, int nt, long long tiles, bool grouped, cudaStream_t st) {
     if (grouped) return nt == 32 ? launch_nt<32, true>(map, a, tiles, st) : nt == 64 ? launch_nt<64, true>(map, a, tiles, st) : launch_nt<128, true>(map, a, tiles, st);

@@ -1,5 +1,5 @@
 // lp_mx_pair.cu - products of packed MXFP4 weights and quantized rows on pairs of SMs (cta_group::2), tiles of 256 weight rows x up to 256 tokens: more
-// than 128 rows of one matrix, or experts with more than 128 pairs on average. Formats and layouts: lp_mx.cu, the instruction: lp_mx_mma.cuh.
+// than 128 rows of one matrix with more tiles than SMs, or experts with more than 128 pairs on average. Formats and layouts: lp_mx.cu, the instruction: lp_mx_mma.cuh.
 //
 // Either CTA of a pair has its 128 weight rows and half of the tokens in shared memory. What bounds one CTA with 128 x 256 is the way from L2, 41 KB a
 // k step of 128 that takes the tensor core 512 cycles; a pair's CTAs take 25 KB each.

@@ -142,7 +142,21 @@ def test_product(M, K, N):
     _close(y, *ref.product(x, v), K, f"M={M} K={K} N={N}")
 
 
-@pytest.mark.parametrize("M", [1, 20, 150, 260])
+@pytest.mark.parametrize("M,K,N", [(640, 4096, 4100), (600, 8192, 2100), (1030, 4096, 2600), (512, 14336, 3900)])
+def test_product_on_pairs_of_sms(M, K, N):
+    """Shapes whose tiles go to pairs of SMs (the workspace then holds parts of cut tiles): odd numbers of row tiles, ragged last tiles of both kinds, k cut."""
+    from laplace_b200 import device
+    assert device.lib().laplace_cuda_mxfp4_workspace_size(M, 0, K, N) > 148 * 2 * 256 * 512
+    rng = np.random.default_rng(912)
+    w = rng.integers(0, 256, (N * K // 32, 17), dtype=np.uint8)
+    w[:, 0] = 118 + w[:, 0] % 6
+    x = _act(913, M, K)
+    y = device.mxfp4_gemm(_dev(x), device.mxfp4_pack(_dev(w.reshape(-1)), N, K), M, K, N)
+    device.sync()
+    _close(y, *ref.product(x, ref.dequantize_mxfp4(w).reshape(N, K)), K, f"M={M} K={K} N={N}")
+
+
+@pytest.mark.parametrize("M", [1, 20, 150, 260, 1000])
 def test_every_value_counts_once(M):
     """Weights that are a single 1 per row: y picks single activations, whose value and place must be right for every k and scale."""
     from laplace_b200 import device
@@ -347,9 +361,12 @@ def _calls(seed):
     we, _ = _blocks(seed + 1, E * N, K)
     packed, experts = device.mxfp4_pack(_dev(w), N, K), device.mxfp4_pack(_dev(we), N, K, E)
     xs = [_dev(_act(seed + 2 + m, m, K)) for m in (1, 50, 300)]
+    big, wide = _dev(_act(seed + 7, 640, 4096)), device.mxfp4_pack(device.mxfp4_quantize(_dev(synth.normal_f32(seed + 8, (4100, 4096)) * 0.02)), 4100, 4096)      # on pairs of SMs
     expert, row = _dev(_routing(seed + 9, 50, E, 3, 1.)), _dev(np.repeat(np.arange(50, dtype=np.int32), 3))
+    many = _dev(_routing(seed + 10, 300, E, 1, 3.))
     return [lambda x=x: device.mxfp4_gemm(x, packed, x.shape[0], K, N) for x in xs] + [
-        lambda: device.mxfp4_moe_grouped(xs[1], experts, expert, row, E, K, N), lambda: device.mxfp4_quantize(xs[2])]
+        lambda: device.mxfp4_moe_grouped(xs[1], experts, expert, row, E, K, N), lambda: device.mxfp4_quantize(xs[2]),
+        lambda: device.mxfp4_gemm(big, wide, 640, 4096, 4100), lambda: device.mxfp4_moe_grouped(xs[2], experts, many, None, E, K, N)]
 
 
 def test_the_same_call_gives_the_same_bits():
