@@ -209,7 +209,7 @@ int launch_act(long long rows, int kts, cudaStream_t st, A... args) {
 // of its own. Its warps have a run of the pairs each, and with the counts of the warps before them they give every pair its place - by
 // its number, not by timing. The counts are made by every block for itself (shared-memory atomics) or, from COUNT_FROM pairs on, by a launch
 // of their own. 2,048 / 16,384 pairs, 128 experts, us under ncu: a warp per expert, 32 of them to a block 24 / 158, one block with match
-// instructions 12 / 27, counts by every block of 1024 threads 7.4 / 19, by a launch 14 / 19; now 6.4 / 5.5 + 10.6.
+// instructions 12 / 27, counts by every block of 1024 threads 7.4 / 19, by a launch 14 / 19; now 5.6 / 5.5 + 8.4.
 constexpr int GROUP_THREADS = 1024;
 constexpr int NO_EXPERT = -1, BAD_EXPERT = -2;
 __device__ __forceinline__ int expert_of(const int* __restrict__ pair_expert, int p, int P, int E) {
@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(GROUP_THREADS) mx_group_kernel(const int* __re
             tab[t0 + i] = make_int4(e, s + (i << tile_log2), min(1 << tile_log2, c - (i << tile_log2)), (t0 + i) * tile_groups);
     }
 }
-// threads of the grouping block: the instructions of all its warps are what the launch waits for (2,048 pairs: 1024 threads 8.7 us, 256 6.4)
+// threads of the grouping block: the instructions of all its warps are what the launch waits for (2,048 pairs: 1024 threads 8.7 us, 256 5.6)
 int group_threads(int pairs) { return pairs < COUNT_FROM ? 256 : GROUP_THREADS; }
 static_assert(COUNT_FROM - 1 <= 256 * 16, "a warp's run of pairs is counted from registers");
 constexpr int MAX_EXPERTS = 4000;          // three words each in the 48 KB of shared memory that a launch may have without asking

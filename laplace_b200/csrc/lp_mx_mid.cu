@@ -6,8 +6,8 @@
 // - CTA o owns the o-th run of the tokens -, which add the parts in the order of k and write y. (Parts through global memory with a
 // counter, the last CTA adding up: 10,000 cycles from the last product to the end, most of it the fence behind the stores and the way
 // back; 77 x 2816 x 8448 13.6 us.)
-// 24 x 14336 x 4096 13.7 us, 77 x 2816 x 8448 10.6, 128 x 4096 x 14336 14.9, quantizer and all; a kernel that only copies 29 MB of weights from cold memory
-// into shared memory takes 7.5. 2,048 pairs of 128 experts 2048 x 1536 (214 MB) 43 us, 4.9 TB/s, 48 with grouping and quantizer.
+// 24 x 14336 x 4096 13.7 us, 77 x 2816 x 8448 10.2, 128 x 4096 x 14336 14.9, 512 x 4096 x 4096 14.9, quantizer and all; a kernel that only copies 29 MB of weights from cold memory
+// into shared memory takes 7.5. 2,048 pairs of 128 experts 2048 x 1536 (214 MB) 42 us, 5 TB/s, 46 with grouping and quantizer.
 //
 // Roles by warp: 0 copies, 1 MMA issue (owns the TMEM), 4-11 drain (lane = weight row), sums and output. All waits are bounded; a wait that
 // gives up raises the status word and the roles leave their loops.
@@ -293,7 +293,7 @@ long long share_k(long long tiles, int kts, int tokens, int& best) {
     for (int i = 0; i < 4; ++i) {
         const int c = 1 << i, n = clusters_of<NT, GROUPED>(i);
         if (!n || kts < c) continue;
-        const long long ns = (tiles + n - 1) / n * ((kts + c - 1) / c * (230 + tokens / 2) + (c > 1 ? 240 * (2 + tokens / 9 + c / 2) : 0));
+        const long long ns = (tiles + n - 1) / n * ((kts + c - 1) / c * (230 + tokens / 2) + (c > 1 ? 900 + 240 * (tokens / 9 + c / 2) : 0));
         if (ns < least) { least = ns; best = i; }
     }
     return least;

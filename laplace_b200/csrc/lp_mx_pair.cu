@@ -13,7 +13,7 @@
 // weight row). All waits are bounded; a wait that gives up raises the status word and the roles leave their loops.
 //
 // 2048 x 14336 x 4096: 540 cycles a step (512 are the tensor core's), 240 Gop in 75 to 87 us under the card's power limit (1.5 GHz), 108 with the quantizer; one
-// CTA with 128 x 256 took 610 cycles a step. 512 x 4096 x 14336 31.8 us, 512 x 4096 x 4096 17.3.
+// CTA with 128 x 256 took 610 cycles a step. 512 x 4096 x 14336 31.9 us, 1000 x 4096 x 14336 55.
 #include "lp_mx.cuh"
 #include "lp_mx_mma.cuh"
 #include "lp_tc.cuh"

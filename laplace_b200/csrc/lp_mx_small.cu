@@ -6,7 +6,7 @@
 // core, out of L2 (M x 512 bytes beside 8.7 KB of weights) - and no sum goes through memory: the CTAs of a cluster share out k, and each sends its
 // part of a tile's results straight into the shared memory of the tile's owner, which adds them in the order of k and writes y.
 //
-// One row: 4096 x 1024 3.6 us, 4096 x 14336 9.8 us (31 MB; a kernel that only copies them from cold memory takes 8), 28672 rows 12.5 us (5 TB/s); eight rows of 4096 x
+// One row: 4096 x 1024 3.25 us, 4096 x 4096 5.5, 4096 x 14336 9.8 us (31 MB; a kernel that only copies them from cold memory takes 8), 28672 rows 12.5 us (5 TB/s); eight rows of 4096 x
 // 14336 10.8. With quantizer launch and sums through global memory 8.2, 17.2 and, eight rows, 18.1. Two CTAs an SM, so that the next call's first copies and the
 // last sums of this one overlap.
 //
@@ -316,7 +316,7 @@ int launch_c(const CUtensorMap& map, SmallArgs a, int tiles, cudaStream_t st) {
 template <bool GROUPED>
 int launch_small(const CUtensorMap& map, const SmallArgs& a, int tiles, cudaStream_t st) {
     // k over C CTAs, so that the time is least: rounds of tiles, each the steps of a CTA (200 ns, or more where so many CTAs are at work that memory is
-    // what they wait for: 470 with all of them) and an exchange. Measured, one row, us with C = 1 / 2 / 4 / 8: 4096 x 1024 8.6 / 5.5 / 4.1 / 3.6, 4096 x 4096
+    // what they wait for: 470 with all of them) and an exchange. Measured, one row, us with C = 1 / 2 / 4 / 8 (with a barrier at the end, 0.3 us): 4096 x 1024 8.6 / 5.5 / 4.1 / 3.6, 4096 x 4096
     // 8.8 / 6.1 / 5.9 / 7.5, 4096 x 14336 9.8 / 10.6 / 11.1 / 14.4, 14336 x 4096 25.5 / 14.7 / 9.8 / 12.6, eight experts 2048 x 1536 6.7 / 7.7 / 7.9 / 6.6.
     const int n[4] = {clusters_of<1, GROUPED>(), clusters_of<2, GROUPED>(), clusters_of<4, GROUPED>(), clusters_of<8, GROUPED>()};
     int best = 0;
