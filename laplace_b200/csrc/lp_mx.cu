@@ -26,27 +26,31 @@ namespace {
 using namespace mx;
 
 // ---- values -> GGUF blocks ---------------------------------------------------------------------------------------
-// A block per 4 lanes, 8 values each; 256 blocks a CTA in four rounds whose loads all go first, gathered in shared memory (a block is 17 bytes) and
-// written in order. 14336 x 4096: fp32 40 us (6.6 TB/s, what a copy reaches), bf16 28.8 us (5.2 TB/s; instructions are 60 % of what the SMs can issue). With
-// one round a CTA 55 and 50.
-constexpr int QROUNDS = 4, QB = 64 * QROUNDS;
-template <class T>
+// A block per 4 lanes, 8 values each; 64 blocks a round, whose loads all go first, gathered in shared memory (a block is 17 bytes) and written in order.
+// us with 2 / 4 / 8 rounds a CTA: 14336 x 4096 bf16 34.7 / 28.9 / 26.5 (5.6 TB/s; instructions are some 60 % of what the SMs can issue), fp32 41.9 / 39.9 / 40.6
+// (6.7 TB/s, what a copy reaches), 1001 x 2848 fp16 2.85 / 3.05 / 3.4, 1 x 4096 1.7 / 1.85 / 2.35. One round and 16-byte stores by half as many lanes: bf16 50, fp32 55.
+constexpr int QB = 64;
+template <class T> int quantize_rounds(long long blocks) {
+    const long long round = static_cast<long long>(QB) * ctx().sm_count;       // an SM's CTAs have a round each
+    return blocks < 16 * round ? 2 : sizeof(T) == 2 && blocks > 64 * round ? 8 : 4;
+}
+template <class T, int ROUNDS>
 __global__ void __launch_bounds__(256) mxfp4_quantize_kernel(const T* __restrict__ x, uint8_t* __restrict__ w, long long n_blocks) {
-    __shared__ __align__(16) uint8_t out[QB * 17];
+    __shared__ __align__(16) uint8_t out[QB * ROUNDS * 17];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int part = threadIdx.x & 3;
-    const long long b0 = static_cast<long long>(blockIdx.x) * QB;
-    const int here = n_blocks - b0 < QB ? static_cast<int>(n_blocks - b0) : QB;
-    Eight<T> in[QROUNDS];
+    const long long b0 = static_cast<long long>(blockIdx.x) * (QB * ROUNDS);
+    const int here = n_blocks - b0 < QB * ROUNDS ? static_cast<int>(n_blocks - b0) : QB * ROUNDS;
+    Eight<T> in[ROUNDS];
 #pragma unroll
-    for (int i = 0; i < QROUNDS; ++i) {
-        const int blk = (threadIdx.x >> 2) + 64 * i;
+    for (int i = 0; i < ROUNDS; ++i) {
+        const int blk = (threadIdx.x >> 2) + QB * i;
         if (blk < here) in[i].load(x + (b0 + blk) * 32 + part * 8);
         else in[i].zero();
     }
 #pragma unroll
-    for (int i = 0; i < QROUNDS; ++i) {
-        const int blk = (threadIdx.x >> 2) + 64 * i;
+    for (int i = 0; i < ROUNDS; ++i) {
+        const int blk = (threadIdx.x >> 2) + QB * i;
         uint32_t a = in[i].amax();
         a = max(a, __shfl_xor_sync(0xffffffffu, a, 1));
         a = max(a, __shfl_xor_sync(0xffffffffu, a, 2));
@@ -81,6 +85,19 @@ __global__ void __launch_bounds__(256) mxfp4_quantize_kernel(const T* __restrict
     } else {
         for (int i = threadIdx.x; i < bytes; i += 256) dst[i] = out[i];
     }
+}
+
+template <class T>
+int launch_quantize(const void* x, uint8_t* w, long long blocks, cudaStream_t st) {
+    const int r = quantize_rounds<T>(blocks);
+    const long long grid = (blocks + QB * r - 1) / (QB * r);
+    if (grid > 0x7fffffffll) return fail(LAPLACE_ERR_LIMIT, "mxfp4_quantize: n=%lld", blocks * 32);
+    const dim3 g(static_cast<unsigned>(grid));
+    const T* p = static_cast<const T*>(x);
+    ctx().launches++;
+    if (r == 2) return launch_early(mxfp4_quantize_kernel<T, 2>, g, 256, 0, st, p, w, blocks);
+    if (sizeof(T) == 2 && r == 8) return launch_early(mxfp4_quantize_kernel<T, 8>, g, 256, 0, st, p, w, blocks);
+    return launch_early(mxfp4_quantize_kernel<T, 4>, g, 256, 0, st, p, w, blocks);
 }
 
 // ---- GGUF blocks -> values (dequantize) ----------------------------------------------------------------------------
@@ -511,14 +528,8 @@ int laplace_cuda_mxfp4_quantize_dev(const void* x, uint32_t x_type, uint8_t* w, 
     if (n == 0) return LAPLACE_OK;
     if (!x || !w || n < 0 || n % 32) return fail(LAPLACE_ERR_ARG, "mxfp4_quantize: n=%lld is not a multiple of 32, or a null pointer", n);
     if (misaligned(x, 16)) return fail(LAPLACE_ERR_ARG, "mxfp4_quantize: x must be 16-byte aligned");
-    const long long blocks = n / 32, grid = (blocks + QB - 1) / QB;
-    if (grid > 0x7fffffffll) return fail(LAPLACE_ERR_LIMIT, "mxfp4_quantize: n=%lld", n);
     cudaStream_t st = MX_STREAM(stream);
-    const dim3 g(static_cast<unsigned>(grid));
-    ctx().launches++;
-    if (x_type == 0) return launch_early(mxfp4_quantize_kernel<float>, g, 256, 0, st, static_cast<const float*>(x), w, blocks);
-    if (x_type == 1) return launch_early(mxfp4_quantize_kernel<__half>, g, 256, 0, st, static_cast<const __half*>(x), w, blocks);
-    return launch_early(mxfp4_quantize_kernel<__nv_bfloat16>, g, 256, 0, st, static_cast<const __nv_bfloat16*>(x), w, blocks);
+    return x_type == 0 ? launch_quantize<float>(x, w, n / 32, st) : x_type == 1 ? launch_quantize<__half>(x, w, n / 32, st) : launch_quantize<__nv_bfloat16>(x, w, n / 32, st);
 }
 
 size_t laplace_cuda_mxfp4_packed_size(int n_experts, int N, int K) {

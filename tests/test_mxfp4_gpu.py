@@ -50,7 +50,7 @@ def _edge_values():
 
 
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
-@pytest.mark.parametrize("shape", [(1, 32), (3, 96), (1, 4096), (65, 2848), (1000, 64)])
+@pytest.mark.parametrize("shape", [(1, 32), (3, 96), (1, 4096), (65, 2848), (1000, 64), (2001, 2848), (1501, 14336)])
 def test_quantize(dtype, shape):
     import torch
     from laplace_b200 import device
