@@ -271,6 +271,8 @@ int laplace_cuda_lm_head_dev(const float* x, const uint8_t* w, uint32_t type, fl
  *   y[p][j] = sum_k xq[pair_row[p]][k] * w[pair_expert[p]][j][k]; pair_row = NULL: pair p reads row p. Pairs in any order. A
  *   negative expert leaves its row of y untouched; an expert >= n_experts_total or a row outside [0, x_rows) does too and
  *   makes the next laplace_cuda_sync() return LAPLACE_ERR_ARG. At most 4000 experts. n_pairs = 0 is a call without effect.
+ * A call takes up to 2^24 rows or pairs, and weights of up to 2^24 - 1 tiles of 128 rows x 128 values, all experts together (more: LAPLACE_ERR_LIMIT,
+ *   and a packed size of 0).
  * K is a multiple of 32, x 16-byte aligned. Workspace: the caller's, laplace_cuda_mxfp4_workspace_size(M or n_pairs, 0 or
  *   n_experts_total, K, N) bytes (after laplace_cuda_init; 0: none is needed, NULL will do, or the sizes are none that a call
  *   takes), 256-byte aligned, its contents of no consequence before or after. Calls with workspaces of their own may overlap,

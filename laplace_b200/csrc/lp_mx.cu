@@ -494,12 +494,13 @@ int launch_product(const float* x, int x_rows, const uint8_t* packed, const int*
     return launch_mx_mid(map, a, p.nt, GROUPED ? static_cast<long long>(experts < rows ? experts : rows) * p.rts : p.share.tiles, GROUPED, st);
 }
 
-// rows: token tiles times row tiles are counted in 32 bits
-bool too_many(long long rows, long long experts, int N) { return (rows / 32 + experts + 1) * ((N + 127) / 128) > 0x3fffffffll; }
+// Limits of a call. Tiles of weights: the tensor map counts their rows of 64 bytes in 31 bits. Rows: token tiles times row tiles are counted in 32 bits.
+long long tiles_of(int n) { return (n + 127ll) / 128; }
+bool too_large(long long experts, int N, int K) { return experts > 0xffffff || experts * tiles_of(N) > 0xffffff || experts * tiles_of(N) * tiles_of(K) > 0xffffff; }
+bool too_many(long long rows, long long experts, int N) { return rows > 1 << 24 || (rows / 32 + experts + 1) * tiles_of(N) > 0x3fffffffll; }
 int bad_shape(const char* what, int K, int N, long long experts) {
     if (K <= 0 || N <= 0 || experts <= 0 || K % 32) return fail(LAPLACE_ERR_ARG, "%s: K=%d (a positive multiple of 32) N=%d experts=%lld", what, K, N, experts);
-    // rows of 64 bytes that the tensor map of the weights counts
-    if (experts * ((N + 127ll) / 128) * ((K + 127) / 128) * 128 > 0x7fffffffll) return fail(LAPLACE_ERR_LIMIT, "%s: %lld x %d x %d values are more than one call takes", what, experts, N, K);
+    if (too_large(experts, N, K)) return fail(LAPLACE_ERR_LIMIT, "%s: %lld x %d x %d values are more than one call takes", what, experts, N, K);
     return LAPLACE_OK;
 }
 bool misaligned(const void* p, unsigned n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }
@@ -533,8 +534,8 @@ int laplace_cuda_mxfp4_quantize_dev(const void* x, uint32_t x_type, uint8_t* w, 
 }
 
 size_t laplace_cuda_mxfp4_packed_size(int n_experts, int N, int K) {
-    if (n_experts <= 0 || N <= 0 || K <= 0 || K % 32) return 0;
-    return static_cast<size_t>(n_experts) * ((N + 127) / 128) * ((K + 127) / 128) * (Q_TILE + SF_TILE);
+    if (n_experts <= 0 || N <= 0 || K <= 0 || K % 32 || too_large(n_experts, N, K)) return 0;
+    return static_cast<size_t>(n_experts * tiles_of(N) * tiles_of(K)) * (Q_TILE + SF_TILE);
 }
 
 int laplace_cuda_mxfp4_pack_dev(const uint8_t* w, uint8_t* packed, int n_experts, int N, int K, void* stream) {
@@ -560,6 +561,7 @@ int laplace_cuda_mxfp4_pack_dev(const uint8_t* w, uint8_t* packed, int n_experts
 
 size_t laplace_cuda_mxfp4_workspace_size(int rows, int n_experts, int K, int N) {
     if (!ctx().ready || rows <= 0 || n_experts < 0 || K <= 0 || N <= 0 || K % 32 || mx_small_takes(rows, n_experts > 0)) return 0;
+    if (n_experts > MAX_EXPERTS || too_large(n_experts ? n_experts : 1, N, K) || too_many(rows, n_experts ? n_experts : 1, N)) return 0;
     return plan_of(rows, n_experts, K, N).bytes;
 }
 
@@ -568,7 +570,7 @@ int laplace_cuda_mxfp4_gemm_dev(const float* x, const uint8_t* packed, float* y,
     if (const int rc = bad_shape("mxfp4_gemm", K, N, 1)) return rc;
     if (M < 0) return fail(LAPLACE_ERR_ARG, "mxfp4_gemm: M=%d", M);
     if (M == 0) return LAPLACE_OK;
-    if (M > 1 << 24 || too_many(M, 1, N)) return fail(LAPLACE_ERR_LIMIT, "mxfp4_gemm: M=%d", M);
+    if (too_many(M, 1, N)) return fail(LAPLACE_ERR_LIMIT, "mxfp4_gemm: M=%d", M);
     const size_t need = laplace_cuda_mxfp4_workspace_size(M, 0, K, N);
     if (!x || !packed || !y || (need && !workspace)) return fail(LAPLACE_ERR_ARG, "mxfp4_gemm: null pointer");
     if (misaligned(x, 16) || misaligned(packed, 128) || misaligned(workspace, 256) || misaligned(y, 4))
@@ -583,7 +585,7 @@ int laplace_cuda_mxfp4_moe_grouped_dev(const float* x, int x_rows, const uint8_t
     if (const int rc = bad_shape("mxfp4_moe_grouped", K, N, n_experts_total)) return rc;
     if (n_pairs < 0 || x_rows < 0) return fail(LAPLACE_ERR_ARG, "mxfp4_moe_grouped: n_pairs=%d x_rows=%d", n_pairs, x_rows);
     if (n_pairs == 0) return LAPLACE_OK;
-    if (n_pairs > 1 << 24 || too_many(n_pairs, n_experts_total, N)) return fail(LAPLACE_ERR_LIMIT, "mxfp4_moe_grouped: n_pairs=%d", n_pairs);
+    if (too_many(n_pairs, n_experts_total, N)) return fail(LAPLACE_ERR_LIMIT, "mxfp4_moe_grouped: n_pairs=%d", n_pairs);
     if (n_experts_total > MAX_EXPERTS) return fail(LAPLACE_ERR_LIMIT, "mxfp4_moe_grouped: %d experts, %d at most", n_experts_total, MAX_EXPERTS);
     const size_t need = laplace_cuda_mxfp4_workspace_size(n_pairs, n_experts_total, K, N);
     if (!x || !packed || !pair_expert || !y || (need && !workspace)) return fail(LAPLACE_ERR_ARG, "mxfp4_moe_grouped: null pointer");

@@ -293,7 +293,7 @@ long long share_k(long long tiles, int kts, int tokens, int& best) {
     for (int i = 0; i < 4; ++i) {
         const int c = 1 << i, n = clusters_of<NT, GROUPED>(i);
         if (!n || kts < c) continue;
-        const long long ns = (tiles + n - 1) / n * ((kts + c - 1) / c * (230 + tokens / 2) + (c > 1 ? 900 + 240 * (tokens / 9 + c / 2) : 0));
+        const long long ns = (tiles + n - 1) / n * ((kts + c - 1) / c * (230ll + tokens / 2) + (c > 1 ? 900 + 240 * (tokens / 9 + c / 2) : 0));
         if (ns < least) { least = ns; best = i; }
     }
     return least;

@@ -88,3 +88,14 @@ def test_gguf_file_with_mxfp4_tensors(tmp_path):
             assert e.kind == 2 and e.experts == (2 * rank, 2 * rank + 2) and e.nbytes == 2 * NE * 34
         finally:
             g.close()
+
+
+def test_sizes_at_the_end_of_the_range():
+    """Tiles are counted in more than 32 bits: 2^24 - 1 of them are the most that a call takes (2^31 rows of packed bytes), above that the size is 0."""
+    L = _lib.load()
+    most = (1 << 24) - 1
+    assert L.laplace_cuda_mxfp4_packed_size(1, most * 128, 32) == most * (128 * 64 + 512)
+    assert L.laplace_cuda_mxfp4_packed_size(1, 1, most * 128) == most * (128 * 64 + 512)
+    assert L.laplace_cuda_mxfp4_packed_size(most, 1, 32) == most * (128 * 64 + 512)
+    for over in ((1, most * 128 + 1, 32), (1, 2 ** 31 - 1, 32), (1, 1, most * 128 + 32), (1, 1, 2 ** 31 - 32), (most + 1, 1, 32), (2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 32)):
+        assert L.laplace_cuda_mxfp4_packed_size(*over) == 0, over

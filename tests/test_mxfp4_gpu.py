@@ -580,3 +580,20 @@ def test_more_pairs_than_one_block_counts_and_bad_rows_among_them():
         ok[bad] = -1
         _close(y, *_grouped_ref(x, v.reshape(E, N, K), ok, np.clip(row, 0, T - 1), y0), K, f"{T}")
         assert torch.equal(y[torch.from_numpy(bad).cuda()], torch.full((len(bad), N), 7.0, device="cuda"))
+
+
+def test_sizes_beyond_the_limits_are_refused():
+    """Each limit of the header: the call says so, and the size of a workspace is 0. No pointer is looked at before."""
+    from laplace_b200 import device
+    L = device.lib()
+    p, K, N = 4096, 2 ** 31 - 32, 1                            # (an address that nothing reads)
+    for rows, experts, k, n in ((1, 0, K, 1), (40, 0, K, 1), (1, 0, 32, 2 ** 31 - 1), (300, 0, 32, 2 ** 31 - 1), ((1 << 24) + 1, 0, 32, 1), (2 ** 31 - 1, 0, 32, 1), (1 << 24, 0, 32, 1 << 20),
+                                (40, 1 << 20, 4096, 128), (40, 4001, 32, 1), ((1 << 24) + 1, 4, 32, 1), (2 ** 31 - 1, 4, 32, 1), (40, 2, K, 1)):
+        assert L.laplace_cuda_mxfp4_workspace_size(rows, experts, k, n) == 0, (rows, experts, k, n)
+        if experts:
+            rc = L.laplace_cuda_mxfp4_moe_grouped_dev(p, 2 ** 31 - 1, p, p, None, rows, experts, p, k, n, p, 1 << 60, 1)
+        else:
+            rc = L.laplace_cuda_mxfp4_gemm_dev(p, p, p, rows, k, n, p, 1 << 60, 1)
+        assert rc == -5, (rows, experts, k, n)
+    assert L.laplace_cuda_mxfp4_pack_dev(p, p, 1, 1, K, 1) == -5 and L.laplace_cuda_mxfp4_pack_dev(p, p, 1, 2 ** 31 - 1, 32, 1) == -5
+    device.sync()
