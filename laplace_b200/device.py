@@ -259,6 +259,11 @@ def _here(*tensors) -> bool:
     return all(t.is_cuda and t.is_contiguous() and t.device.index == torch.cuda.current_device() for t in tensors if t is not None)
 
 
+def _sizes(*values: int) -> bool:
+    """Whether they are sizes that an int of the ABI holds: ctypes would cut them to 32 bits without a word."""
+    return all(-2 ** 31 <= v < 2 ** 31 for v in values)
+
+
 def mxfp4_quantize(x: torch.Tensor, w: torch.Tensor | None = None) -> torch.Tensor:
     """Values (fp32, fp16 or bf16; rows a multiple of 32 long) -> MXFP4 blocks as GGUF holds them, flat bytes
     (laplace_cuda_mxfp4_quantize_dev). dequantize, embed_rows and mxfp4_pack take them."""
@@ -279,7 +284,7 @@ def mxfp4_pack(w: torch.Tensor, N: int, K: int, n_experts: int = 1) -> torch.Ten
     """GGUF MXFP4 blocks of n_experts matrices [N][K] -> the layout that mxfp4_gemm and mxfp4_moe_grouped read
     (laplace_cuda_mxfp4_pack_dev): once, when the weights are loaded."""
     L = lib()
-    assert w.dtype == torch.uint8 and _here(w) and w.numel() >= n_experts * N * any_row_bytes(39, K)
+    assert _sizes(N, K, n_experts) and w.dtype == torch.uint8 and _here(w) and w.numel() >= n_experts * N * any_row_bytes(39, K)
     packed = torch.empty(L.laplace_cuda_mxfp4_packed_size(n_experts, N, K), dtype=torch.uint8, device=w.device)
     _check(L, L.laplace_cuda_mxfp4_pack_dev(w.data_ptr(), packed.data_ptr(), n_experts, N, K, _stream()))
     return packed
@@ -291,7 +296,7 @@ def mxfp4_gemm(x: torch.Tensor, packed: torch.Tensor, M: int, K: int, N: int, y:
     if r is not None:
         return r
     L = lib()
-    assert x.dtype == torch.float32 and packed.dtype == torch.uint8 and _here(x, packed, y) and M >= 0 and x.numel() >= M * K
+    assert _sizes(M, K, N) and x.dtype == torch.float32 and packed.dtype == torch.uint8 and _here(x, packed, y) and M >= 0 and x.numel() >= M * K
     assert packed.numel() >= L.laplace_cuda_mxfp4_packed_size(1, N, K)
     if y is None:
         y = torch.empty((M, N), dtype=torch.float32, device=x.device)
@@ -310,7 +315,7 @@ def mxfp4_moe_grouped(x: torch.Tensor, packed: torch.Tensor, pair_expert: torch.
         return r
     L = lib()
     P = pair_expert.numel()
-    assert K > 0 and pair_expert.dtype == torch.int32 and (pair_row is None or (pair_row.dtype == torch.int32 and pair_row.numel() == P))
+    assert _sizes(P, x.numel() // K if K > 0 else K, n_experts_total, K, N) and K > 0 and pair_expert.dtype == torch.int32 and (pair_row is None or (pair_row.dtype == torch.int32 and pair_row.numel() == P))
     assert x.dtype == torch.float32 and packed.dtype == torch.uint8 and _here(x, packed, pair_expert, pair_row, y)
     assert packed.numel() >= L.laplace_cuda_mxfp4_packed_size(n_experts_total, N, K)
     if y is None:

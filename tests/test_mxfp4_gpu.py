@@ -597,3 +597,21 @@ def test_sizes_beyond_the_limits_are_refused():
         assert rc == -5, (rows, experts, k, n)
     assert L.laplace_cuda_mxfp4_pack_dev(p, p, 1, 1, K, 1) == -5 and L.laplace_cuda_mxfp4_pack_dev(p, p, 1, 2 ** 31 - 1, 32, 1) == -5
     device.sync()
+
+
+def test_sizes_above_32_bits_are_refused():
+    """2^32 more than a right size is not that size."""
+    import torch
+    from laplace_b200 import device
+    K, N, E = 64, 40, 2
+    w, _ = _blocks(1500, E * N, K)
+    w, x = _dev(w), _dev(_act(1501, 4, K))
+    packed, one, expert = device.mxfp4_pack(w, N, K, E), device.mxfp4_pack(w, N, K), torch.zeros(4, dtype=torch.int32, device="cuda")
+    big = 2 ** 32
+    wide = torch.empty((big + K) // 32 * 17, dtype=torch.uint8, device="cuda")      # a row of 2^32 + 64 values
+    for bad in (lambda: device.mxfp4_pack(wide, 1, big + K), lambda: device.mxfp4_gemm(x, one, 1, K, big + N), lambda: device.mxfp4_gemm(x, one, 0, big + K, N),
+                lambda: device.mxfp4_moe_grouped(x, packed, expert, None, big + E, K, N), lambda: device.mxfp4_moe_grouped(x, packed, expert[:1], None, E, K, big + N),
+                lambda: device.mxfp4_moe_grouped(x, packed, expert[:0], None, E, big + K, N)):
+        with pytest.raises(AssertionError):
+            bad()
+    device.sync()
