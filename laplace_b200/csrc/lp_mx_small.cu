@@ -119,11 +119,14 @@ __global__ void __launch_bounds__(THREADS, 2) mx_small_kernel(const __grid_const
     const int k0 = a.kts * rank / C, k1 = a.kts * (rank + 1) / C;      // every CTA has a step at least: kts >= C
 
     if (warp == 0 && elect_one()) {
-        int st = 0, parity = 1;
+        // One matrix: a ring of weights may be copied while the kernel before this one ends. Nothing is freed before it has (the quantizers wait for it), however
+        // long that takes, so the bounded waits begin after it.
+        int st = 0, parity = 1, early = GROUPED ? 0 : S;
         bool ok = true;
         for (int t = cluster; ok && t < tiles; t += clusters) {
             const size_t tile0 = (static_cast<size_t>(f.expert[t / a.rts]) * a.rts + t % a.rts) * a.kts;
             for (int kt = k0; kt < k1; ++kt) {
+                if (!GROUPED && early-- == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
                 if (!wait_or_abort<false>(bar(f.empty[st]), parity, abort_flag, a.err, DEV_TIMEOUT_EMPTY)) { ok = false; break; }
                 const uint32_t b = bar(f.full[st]);
                 mbar_expect_tx(b, Q_TILE + SF_TILE);
@@ -138,6 +141,7 @@ __global__ void __launch_bounds__(THREADS, 2) mx_small_kernel(const __grid_const
     } else if (warp == 1 && elect_one()) {
         int st = 0, parity = 0, i = 0, set = 0;      // set: of TMEM columns for the scales
         bool ok = true;
+        if (!GROUPED) asm volatile("griddepcontrol.wait;" ::: "memory");
         for (int t = cluster; ok && t < tiles; t += clusters, ++i) {
             const int acc = i % ACCS;
             if (i >= ACCS && !wait_or_abort<true>(bar(f.tempty[acc]), (i / ACCS - 1) & 1, abort_flag, a.err, DEV_TIMEOUT_TMEM)) break;

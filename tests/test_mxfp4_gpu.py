@@ -615,3 +615,23 @@ def test_sizes_above_32_bits_are_refused():
         with pytest.raises(AssertionError):
             bad()
     device.sync()
+
+
+def test_products_right_behind_a_long_kernel():
+    """A kernel of some milliseconds that lets the next one start early, and a product of its results behind it: the same bits as with a pause in between."""
+    import torch
+    from laplace_b200 import device
+    M, K, N = 4096, 4096, 4096
+    q = device.upload_weights(synth.weights(GGMLType.Q4_K, K, N, seed=1510, how="affine"))
+    w, _ = _blocks(1511, 600, N)
+    packed = device.mxfp4_pack(_dev(w), 600, N)
+    x = _dev(_act(1512, M, K))
+    for rows in (1, 8, 40, 300):
+        got = []
+        for pause in (True, False, False):
+            h = device.gemm(x, q, GGMLType.Q4_K, M, K, N)
+            if pause:
+                torch.cuda.synchronize()
+            got.append(device.mxfp4_gemm(h[M - rows:], packed, rows, N, 600))
+        device.sync()
+        assert torch.isfinite(got[0]).all() and torch.equal(got[0], got[1]) and torch.equal(got[0], got[2]), rows
