@@ -289,6 +289,9 @@ int    laplace_cuda_mxfp4_gemm_dev(const float* x, const uint8_t* packed, float*
 int    laplace_cuda_mxfp4_moe_grouped_dev(const float* x, int x_rows, const uint8_t* packed, const int* pair_expert,
                                           const int* pair_row, int n_pairs, int n_experts_total, float* y, int K, int N,
                                           void* workspace, size_t workspace_bytes, void* stream);
+/* Which kernel the last product launched ran on: 1 = up to 8 rows or 32 pairs, 2 = tiles on single SMs, 3 = tiles on pairs of SMs; and 16 times the number
+ * of CTAs that share out k of a tile (on pairs of SMs 1). For tests. */
+int    laplace_cuda_mxfp4_last_kernel(void);
 
 /* ---- row-split prefill: the GEMM stores into every GPU's buffer --------------------------
  * laplace_cuda_gemm_peers_dev is laplace_cuda_gemm_dev for M > 8 over a weight matrix split along N: this GPU's

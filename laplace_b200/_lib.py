@@ -51,6 +51,7 @@ SYMBOLS = {
     "laplace_cuda_mxfp4_workspace_size": (_sz, [_i, _i, _i, _i]),
     "laplace_cuda_mxfp4_gemm_dev": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp, _sz, _vp]),
     "laplace_cuda_mxfp4_moe_grouped_dev": (_i, [_vp, _i, _vp, _vp, _vp, _i, _i, _vp, _i, _i, _vp, _sz, _vp]),
+    "laplace_cuda_mxfp4_last_kernel": (_i, []),
     "laplace_cuda_gguf_open": (_i, [C.c_char_p, _i, _i, C.POINTER(C.c_char_p), _i, C.POINTER(_vp)]),
     "laplace_cuda_gguf_upload": (_i, [_vp]),
     "laplace_cuda_gguf_tensor_count": (_i, [_vp]),

@@ -49,6 +49,7 @@ struct Context {
     int*         h_err = nullptr;      // host view of the same word (mapped pinned memory)
     int          last_path = 0;
     int          last_kernel = 0;      // KERNEL_*
+    int          last_mx = 0;          // laplace_cuda_mxfp4_last_kernel
     long long    launches = 0;
 };
 enum : int { KERNEL_DP4A = 1, KERNEL_INT8 = 2, KERNEL_INT8_TILES = 3, KERNEL_TCGEN05 = 4, KERNEL_TCGEN05_TWO_PIECE = 5, KERNEL_F32ACT = 6,

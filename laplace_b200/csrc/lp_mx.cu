@@ -565,6 +565,8 @@ size_t laplace_cuda_mxfp4_workspace_size(int rows, int n_experts, int K, int N) 
     return plan_of(rows, n_experts, K, N).bytes;
 }
 
+int laplace_cuda_mxfp4_last_kernel(void) { return ctx().last_mx; }
+
 int laplace_cuda_mxfp4_gemm_dev(const float* x, const uint8_t* packed, float* y, int M, int K, int N, void* workspace, size_t workspace_bytes, void* stream) {
     MX_READY();
     if (const int rc = bad_shape("mxfp4_gemm", K, N, 1)) return rc;

@@ -12,6 +12,9 @@ namespace mx {
 constexpr int Q_TILE = 128 * 64;      // bytes of 128 rows x 128 e2m1 values
 constexpr int SF_TILE = 512;          // bytes of their scales: 128 rows x 4
 
+// laplace_cuda_mxfp4_last_kernel: one of these, and 16 times the CTAs that share out k
+enum : int { KERNEL_SMALL = 1, KERNEL_SINGLE = 2, KERNEL_PAIR = 3 };
+
 // Where quantized activations go: the image and its scales, rows in the image, 128-row groups of scales. A token tile's scales
 // begin with a group of their own (the tensor core takes them from TMEM columns whose number is a multiple of four).
 struct ActDst { uint8_t* img; uint8_t* sf; int rows, groups, tile_w, tile_groups; };

@@ -307,6 +307,7 @@ int launch_nt(const CUtensorMap& map, const MxArgs& a, long long tiles, cudaStre
     cudaLaunchConfig_t cfg = config(C, attr, st);
     cfg.gridDim = dim3(clusters_of<NT, GROUPED>(best) * C);
     ctx().launches++;
+    ctx().last_mx = KERNEL_SINGLE + 16 * C;
     return cuda_check(C > 1 ? cudaLaunchKernelEx(&cfg, mx_mid_kernel<NT, GROUPED, true>, map, a, C, stages_of<NT>(C))
                             : cudaLaunchKernelEx(&cfg, mx_mid_kernel<NT, GROUPED, false>, map, a, C, stages_of<NT>(C)), "mx_mid launch");
 }

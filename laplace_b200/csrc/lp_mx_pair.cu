@@ -364,6 +364,7 @@ int launch(const CUtensorMap& map, const MxArgs& a, cudaStream_t st) {
     attr[1].val.clusterDim.x = 2; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cfg.gridDim = dim3(ctx().sm_count / 2 * 2); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = Lay::BYTES; cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = 2;
     ctx().launches++;
+    ctx().last_mx = KERNEL_PAIR + 16;
     return cuda_check(cudaLaunchKernelEx(&cfg, mx_pair_kernel<GROUPED>, map, a), "mx_pair launch");
 }
 

@@ -314,6 +314,7 @@ int launch_c(const CUtensorMap& map, SmallArgs a, int tiles, cudaStream_t st) {
     attr[1].val.clusterDim = {C, 1, 1};
     cfg.gridDim = dim3((tiles < most ? tiles : most) * C); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = SMEM; cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = C > 1 ? 2 : 1;
     ctx().launches++;
+    ctx().last_mx = KERNEL_SMALL + 16 * C;
     return cuda_check(cudaLaunchKernelEx(&cfg, mx_small_kernel<C, GROUPED>, map, a), "mx_small launch");
 }
 
