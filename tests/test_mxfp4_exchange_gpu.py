@@ -1,5 +1,6 @@
-"""MXFP4 products whose k is shared by several CTAs: sums sent through a cluster's shared memory, in kernels of a handful of rows and of middle sizes. Sizes at which
-buffers, slots and accumulators are used again, and tiles are more than a call's plan reckons with; each says which kernel it has to reach."""
+"""MXFP4 products whose k is shared by several CTAs: sums sent through a cluster's shared memory, in kernels of a handful of rows and of middle sizes, and parts of
+cut tiles left in the workspace, on pairs of SMs. Sizes at which buffers, slots and accumulators are used again, runs lie across a tile's border, and tiles are more
+than a call's plan reckons with; each says which kernel it has to reach."""
 import numpy as np
 import pytest
 
@@ -9,6 +10,7 @@ from tests.test_mxfp4_gpu import _act, _close, _dev
 
 pytestmark = pytest.mark.gpu
 SMALL, SINGLE, PAIR = 1, 2, 3                                  # laplace_cuda_mxfp4_last_kernel, + 16 x the CTAs that share k
+MARK = 0xA5
 
 
 def _weights(seed, rows, K):
@@ -149,3 +151,149 @@ def test_pairs_of_middle_sizes(counts, K, N, C, form):
         for _ in range(5):
             assert torch.equal(device.mxfp4_moe_grouped(_dev(x), packed, *args, y=y0.clone()), y)
         device.sync()
+
+
+# ---- cut tiles -----------------------------------------------------------------------------------------------------------------
+
+def _round256(n):
+    return (n + 255) & ~255
+
+
+def _parts_left(ws, behind=0):
+    """Parts of cut tiles that the even CTAs left in a workspace whose last `behind` bytes come after their area: of every cut tile all but the one whose pair was the last.
+    Two slots a pair of SMs, 128 KB for each of its CTAs."""
+    from laplace_b200 import device
+    area = 2 * device.lib().laplace_cuda_sm_count() * 256 * 128 * 4
+    end = ws.numel() - behind
+    return int((ws[end - area:end].view(-1, 2, 256 * 128 * 4)[:, 0] != MARK).any(1).sum())
+
+
+# 300: 18 tiles in four; 600, 2000: 36 and 33 tiles in halves; 2048 x 2600: 14 tiles over 74 pairs of SMs, whose runs lie across the tiles' borders, then 74 whole ones;
+# 1030: 6 tiles in twelve parts and more, then 74 whole ones; 640: none
+@pytest.mark.parametrize("M,K,N,parts", [(300, 14336, 2100, 54), (600, 14336, 2100, 36), (2000, 8192, 700, 33), (2048, 14336, 2600, 72), (1030, 14336, 4096, 72), (640, 4096, 4100, 0)])
+def test_cut_tiles(M, K, N, parts):
+    import torch
+    from laplace_b200 import device
+    L = device.lib()
+    w = _weights(1640 + M, N, K)
+    x = _act(1641 + M, M, K)
+    packed, xd = device.mxfp4_pack(w, N, K), _dev(x)
+    n = L.laplace_cuda_mxfp4_workspace_size(M, 0, K, N)
+    ws, y = torch.full((n,), MARK, dtype=torch.uint8, device="cuda"), torch.empty(M, N, device="cuda")
+    assert L.laplace_cuda_mxfp4_gemm_dev(xd.data_ptr(), packed.data_ptr(), y.data_ptr(), M, K, N, ws.data_ptr(), n, 1) == 0
+    device.sync()
+    assert _kernel() == PAIR + 16 and _parts_left(ws) == parts
+    _close(y, *_product(torch.from_numpy(ref.mxfp8(x)).cuda(), w, N, K), K, f"M={M} K={K} N={N}")
+    for _ in range(5):
+        assert torch.equal(device.mxfp4_gemm(xd, packed, M, K, N), y)
+    device.sync()
+
+
+# The plan is made on the GPU: 12 tiles in three; 24 in three, three experts; 10 in four, of ragged experts and an odd number of row tiles; 14 over 74 pairs of SMs, across the
+# tiles' borders, then 74 whole ones
+@pytest.mark.parametrize("counts,K,N,parts", [((150,), 8192, 3000, 24), ((300, 290, 400), 8192, 1000, 48), ((512, 0, 300, 150), 14336, 300, 30), ((450, 450), 5376, 5600, 72)])
+@pytest.mark.parametrize("form", ["own", "elsewhere", "bad rows"])
+def test_cut_tiles_of_experts(counts, K, N, parts, form):
+    import torch
+    from laplace_b200 import device
+    from laplace_b200.matmul import LaplaceCudaError
+    L = device.lib()
+    E, P = len(counts), sum(counts)
+    rng = np.random.default_rng(1650)
+    expert = rng.permutation(np.repeat(np.arange(E), counts)).astype(np.int32)
+    row, X = None, P
+    if form != "own":
+        X = 33
+        row = rng.integers(0, X, P).astype(np.int32)
+    if form == "elsewhere":
+        expert[::50] = -2
+    ok = expert.copy()
+    if form == "bad rows":
+        row[3::11], ok[3::11] = -1, -1
+    w = _weights(1651 + P, E * N, K)
+    x = _act(1652 + P, X, K)
+    packed, xd, ed = device.mxfp4_pack(w, N, K, E), _dev(x), _dev(expert)
+    rd = None if row is None else _dev(row)
+    n = L.laplace_cuda_mxfp4_workspace_size(P, E, K, N)
+    y0 = torch.full((P, N), 7.0, device="cuda")
+    ws, y = torch.full((n,), MARK, dtype=torch.uint8, device="cuda"), y0.clone()
+    assert L.laplace_cuda_mxfp4_moe_grouped_dev(xd.data_ptr(), X, packed.data_ptr(), ed.data_ptr(), None if rd is None else rd.data_ptr(), P, E, y.data_ptr(), K, N, ws.data_ptr(), n, 1) == 0
+    if form == "bad rows":
+        with pytest.raises(LaplaceCudaError):
+            device.sync()
+    device.sync()
+    # behind the parts: places, rows of results, token tiles, the plan, counts
+    rows, tiles = (P + 7 * min(E, P) + 7) & ~7, P // 256 + min(E, P)
+    behind = _round256(8 * P) + _round256(4 * rows) + _round256(16 * tiles) + 256 + _round256(4 * E)
+    assert _kernel() == PAIR + 16 and _parts_left(ws, behind) == parts
+    _close(y, *_experts(x, w, ok, row, E, N, K, y0.cpu().numpy()), K, f"{counts} K={K} N={N} {form}")
+    if form != "bad rows":
+        for _ in range(5):
+            assert torch.equal(device.mxfp4_moe_grouped(xd, packed, ed, rd, E, K, N, y=y0.clone()), y)
+        device.sync()
+
+
+# ---- side by side ------------------------------------------------------------------------------------------------------------------
+
+def _calls(seed):
+    """Calls that share k in every way, on data of their own: clusters of two kernels, one matrix and experts, more tiles than clusters, cut tiles before whole ones."""
+    from laplace_b200 import device
+
+    def dense(M, K, N):
+        x, p = _dev(_act(seed + M, M, K)), device.mxfp4_pack(_weights(seed + N, N, K), N, K)
+        return lambda: device.mxfp4_gemm(x, p, M, K, N)
+
+    def experts(counts, K, N):
+        expert = np.random.default_rng(seed).permutation(np.repeat(np.arange(len(counts)), counts)).astype(np.int32)
+        x, p, e = _dev(_act(seed + K, len(expert), K)), device.mxfp4_pack(_weights(seed + N, len(counts) * N, K), N, K, len(counts)), _dev(expert)
+        return lambda: device.mxfp4_moe_grouped(x, p, e, None, len(counts), K, N)
+
+    return [dense(2, 4096, 76700), dense(4, 14336, 4096), experts((3, 3, 3, 3), 2048, 512), dense(24, 14336, 10240), experts((129, 65, 1, 61), 4096, 1000), dense(1030, 14336, 2048),
+            dense(300, 14336, 2100), experts((450, 450), 5376, 5600)]
+
+
+def test_streams_side_by_side():
+    import torch
+    from laplace_b200 import device
+    sets = [_calls(1660), _calls(1670)]
+    want = [[f() for f in c] for c in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for turn in range(10):
+        for i in range(len(sets[0])):
+            for side in (0, 1):
+                with torch.cuda.stream(streams[side]):
+                    got[side].append(sets[side][(i + side * turn) % len(sets[0])]())      # other calls meet each turn
+    torch.cuda.synchronize()
+    for side in (0, 1):
+        for turn in range(10):
+            for i in range(len(sets[0])):
+                assert torch.equal(got[side][turn * len(sets[0]) + i], want[side][(i + side * turn) % len(sets[0])])
+    device.sync()
+
+
+def test_two_graphs_replayed_side_by_side():
+    import torch
+    from laplace_b200 import device
+    sets = [_calls(1680), _calls(1690)]
+    want = [[f() for f in c] for c in sets]
+    torch.cuda.synchronize()
+    graphs, outs, streams = [], [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for c in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append([f() for f in c])
+        graphs.append(g)
+    for _ in range(5):
+        for o in outs:
+            for y in o:
+                y.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+                g.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert all(torch.equal(y, z) for y, z in zip(o, w))
+    device.sync()
