@@ -635,3 +635,24 @@ def test_products_right_behind_a_long_kernel():
             got.append(device.mxfp4_gemm(h[M - rows:], packed, rows, N, 600))
         device.sync()
         assert torch.isfinite(got[0]).all() and torch.equal(got[0], got[1]) and torch.equal(got[0], got[2]), rows
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_quantize_edges_of_16_bits(dtype):
+    """Zeros, numbers below the normal ones, the largest ones, ties, infinities and NaN in the types that have a way of their own to the largest magnitude; then every
+    number of the type as its block's largest."""
+    import torch
+    from laplace_b200 import device
+    t = getattr(torch, dtype)
+    info = torch.finfo(t)
+    edges = torch.from_numpy(_edge_values()).clamp(-info.max, info.max).to(t)
+    tiny = torch.tensor([info.smallest_normal, info.smallest_normal / 2, info.smallest_normal * info.eps, 3 * info.smallest_normal * info.eps, info.max, -info.max, info.max / 2], dtype=torch.float64).to(t)
+    bad = torch.ones(4, 32, dtype=t)
+    bad[0, 0], bad[1, 31], bad[2, 16], bad[3, 15] = float("inf"), -float("inf"), float("nan"), -float("nan")
+    every = torch.arange(1 << 16, dtype=torch.int32).to(torch.int16).view(t)
+    g = torch.Generator().manual_seed(1520)
+    blocks = (every.float()[:, None] * torch.rand(1 << 16, 32, generator=g)).to(t)
+    blocks[torch.arange(1 << 16), torch.arange(1 << 16) % 32] = every
+    for x in (edges, tiny[:, None].expand(-1, 32).contiguous(), torch.cat([tiny, -tiny, torch.zeros(18, dtype=t)])[None].contiguous(), bad, blocks):
+        got = device.mxfp4_quantize(x.cuda()).cpu().numpy().reshape(-1, 17)
+        assert np.array_equal(got, ref.quantize_mxfp4(x.float().numpy()).reshape(-1, 17))
