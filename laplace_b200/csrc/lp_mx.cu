@@ -96,7 +96,8 @@ int launch_quantize(const void* x, uint8_t* w, long long blocks, cudaStream_t st
     const T* p = static_cast<const T*>(x);
     ctx().launches++;
     if (r == 2) return launch_early(mxfp4_quantize_kernel<T, 2>, g, 256, 0, st, p, w, blocks);
-    if (sizeof(T) == 2 && r == 8) return launch_early(mxfp4_quantize_kernel<T, 8>, g, 256, 0, st, p, w, blocks);
+    if constexpr (sizeof(T) == 2)
+        if (r == 8) return launch_early(mxfp4_quantize_kernel<T, 8>, g, 256, 0, st, p, w, blocks);
     return launch_early(mxfp4_quantize_kernel<T, 4>, g, 256, 0, st, p, w, blocks);
 }
 
