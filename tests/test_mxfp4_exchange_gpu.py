@@ -297,3 +297,54 @@ def test_two_graphs_replayed_side_by_side():
         for o, w in zip(outs, want):
             assert all(torch.equal(y, z) for y, z in zip(o, w))
     device.sync()
+
+
+# ---- first calls of a process --------------------------------------------------------------------------------------------------------
+
+_FIRST = """
+import sys, threading
+import torch
+from laplace_b200 import device
+from tests.test_mxfp4_exchange_gpu import _calls
+from tests.test_mxfp4_gpu import _calls as _more
+
+sets = [_calls(1700 + 10 * i) + _more(1750 + 10 * i) for i in range({threads})]
+torch.cuda.synchronize()
+"""
+_CAPTURE = _FIRST + """
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    outs = [f() for f in sets[0]]
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(y, f()) for y, f in zip(outs, sets[0]))
+device.sync()
+print("same")
+"""
+_THREADS = _FIRST + """
+got, start = [[] for _ in sets], threading.Barrier(len(sets))
+def work(i):
+    start.wait()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        for _ in range(5):
+            for f in sets[i]:
+                got[i].append(f())
+        torch.cuda.current_stream().synchronize()
+threads = [threading.Thread(target=work, args=(i,)) for i in range(len(sets))]
+[t.start() for t in threads]
+[t.join() for t in threads]
+for ys, calls in zip(got, sets):
+    assert len(ys) == 5 * len(calls) and all(torch.equal(y, calls[i % len(calls)]()) for i, y in enumerate(ys))
+device.sync()
+print("same")
+"""
+
+
+@pytest.mark.parametrize("code,threads", [(_CAPTURE, 1), (_THREADS, 4)], ids=["captured", "threads"])
+def test_first_calls(code, threads):
+    """A process whose first products are captured into a graph, and one whose first products come from several threads at once: results as later."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    r = subprocess.run([sys.executable, "-c", code.replace("{threads}", str(threads))], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0 and r.stdout.strip().endswith("same"), r.stdout + r.stderr
