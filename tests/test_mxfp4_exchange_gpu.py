@@ -348,3 +348,21 @@ def test_first_calls(code, threads):
     from pathlib import Path
     r = subprocess.run([sys.executable, "-c", code.replace("{threads}", str(threads))], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=240)
     assert r.returncode == 0 and r.stdout.strip().endswith("same"), r.stdout + r.stderr
+
+
+# ---- experts whose rows end inside a k tile --------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("tokens", [1, 8, 9, 20, 64, 257, 1100])
+@pytest.mark.parametrize("gate_up", [True, False])
+def test_top_4_of_32_experts_of_2880(tokens, gate_up):
+    """Rows of 22.5 k tiles, four experts a token, from one token to a prompt: gate / up with a row per token, down with a row per pair."""
+    import torch
+    from laplace_b200 import device
+    E, K, N = 32, 2880, 720 if gate_up else 360
+    rng = np.random.default_rng(1720 + tokens)
+    expert = np.argsort(-(rng.standard_normal((tokens, E)) + 1.5 * rng.standard_normal(E)), axis=1)[:, :4].astype(np.int32).reshape(-1)
+    row = np.repeat(np.arange(tokens, dtype=np.int32), 4) if gate_up else None
+    w, x = _weights(1721, E * N, K), _act(1722, tokens if gate_up else 4 * tokens, K)
+    y = device.mxfp4_moe_grouped(_dev(x), device.mxfp4_pack(w, N, K, E), _dev(expert), None if row is None else _dev(row), E, K, N)
+    device.sync()
+    _close(y, *_experts(x, w, expert, row, E, N, K, np.zeros((4 * tokens, N))), K, f"{tokens} tokens")
