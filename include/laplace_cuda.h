@@ -265,7 +265,8 @@ int laplace_cuda_lm_head_dev(const float* x, const uint8_t* w, uint32_t type, fl
  * laplace_cuda_mxfp4_packed_size / _pack_dev: n_experts matrices of N rows of K values (one after the other; w at any
  *   alignment; one matrix: n_experts = 1) -> the packed layout, 128-byte aligned, 0.53 bytes per value and row tiles of 128.
  * laplace_cuda_mxfp4_gemm_dev: y[m][j] = sum_k xq[m][k] * w[j][k], where xq holds x as MXFP8: e4m3 values and, per 32 of them,
- *   the smallest power of two that keeps the largest magnitude within 448 times it, rounded to nearest even. Sums in fp32 (a
+ *   the smallest power of two that keeps the largest magnitude within 448 times it, rounded to nearest even: that moves y by 2.6 % of its norm from
+ *   fp32 activations (normal values; Q8 activations of the other types 0.5 to 0.7 %, 4-bit weights themselves 11 %). Sums in fp32 (a
  *   partial sum that leaves its range is infinite, whatever follows). A block of x with an infinity or a NaN makes its row of y NaN, as a NaN block of the weights makes its column. M = 0 is a call without effect.
  * laplace_cuda_mxfp4_moe_grouped_dev: the same for (token, expert) pairs, as laplace_cuda_moe_grouped_dev:
  *   y[p][j] = sum_k xq[pair_row[p]][k] * w[pair_expert[p]][j][k]; pair_row = NULL: pair p reads row p. Pairs in any order. A

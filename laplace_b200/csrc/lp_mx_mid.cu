@@ -1,13 +1,13 @@
-// lp_mx_mid.cu - products of packed MXFP4 weights and quantized rows, tiles of 128 weight rows x up to 128 tokens: 9 rows of one matrix and more, while its
-// tiles fit on the SMs at once, or experts with up to 128 pairs on average. Formats and layouts: lp_mx.cu, the instruction: lp_mx_mma.cuh.
+// lp_mx_mid.cu - products of packed MXFP4 weights and quantized rows, tiles of 128 weight rows x up to 128 tokens: 9 to 128 rows of one matrix, more where the model
+// of its time is below that of the pairs of SMs (plan_of in lp_mx.cu), or experts with up to 128 pairs on average. Formats and layouts: lp_mx.cu, the instruction: lp_mx_mma.cuh.
 //
 // Bound by the weights' way from memory. A cluster of C CTAs takes tiles number cluster, cluster + clusters, ...; its CTAs share out k where there are
 // fewer tiles than SMs, and C is 1 where there are enough. A CTA sends its part of a tile's results into the shared memory of their owners
 // - CTA o owns the o-th run of the tokens -, which add the parts in the order of k and write y. (Parts through global memory with a
 // counter, the last CTA adding up: 10,000 cycles from the last product to the end, most of it the fence behind the stores and the way
 // back; 77 x 2816 x 8448 13.6 us.)
-// 24 x 14336 x 4096 13.7 us, 77 x 2816 x 8448 10.2, 128 x 4096 x 14336 14.9, 512 x 4096 x 4096 14.9, quantizer and all; a kernel that only copies 29 MB of weights from cold memory
-// into shared memory takes 7.5. 2,048 pairs of 128 experts 2048 x 1536 (214 MB) 42 us, 5 TB/s, 46 with grouping and quantizer.
+// In a graph over weights from cold memory, quantizer and all: 24 x 14336 x 4096 13.8 us, 77 x 2816 x 8448 10.5, 128 x 4096 x 14336 14.9, 512 x 4096 x 4096 14.9; a kernel that only copies 29 MB
+// of weights into shared memory takes 7.5. 2,048 pairs of 128 experts 2048 x 1536 (214 MB) 42 us, 5 TB/s, 46 with grouping and quantizer, 47 to 49 call by call.
 //
 // Roles by warp: 0 copies, 1 MMA issue (owns the TMEM), 4-11 drain (lane = weight row), sums and output. All waits are bounded; a wait that
 // gives up raises the status word and the roles leave their loops.

@@ -1,5 +1,5 @@
 // lp_mx_pair.cu - products of packed MXFP4 weights and quantized rows on pairs of SMs (cta_group::2), tiles of 256 weight rows x up to 256 tokens: more
-// than 128 rows of one matrix with more tiles than SMs, or experts with more than 128 pairs on average. Formats and layouts: lp_mx.cu, the instruction: lp_mx_mma.cuh.
+// than 128 rows of one matrix where the model of its time is below that of single SMs (plan_of in lp_mx.cu), or experts with more than 128 pairs on average. Formats and layouts: lp_mx.cu, the instruction: lp_mx_mma.cuh.
 //
 // Either CTA of a pair has its 128 weight rows and half of the tokens in shared memory. What bounds one CTA with 128 x 256 is the way from L2, 41 KB a
 // k step of 128 that takes the tensor core 512 cycles; a pair's CTAs take 25 KB each.
@@ -12,8 +12,8 @@
 // Roles by warp: 0 copies, 1 MMA issue in the even CTA (owns the TMEM), word of the filled stages in the odd one, 4-11 drain (lane =
 // weight row). All waits are bounded; a wait that gives up raises the status word and the roles leave their loops.
 //
-// 2048 x 14336 x 4096: 540 cycles a step (512 are the tensor core's), 240 Gop in 75 to 87 us under the card's power limit (1.5 GHz), 108 with the quantizer; one
-// CTA with 128 x 256 took 610 cycles a step. 512 x 4096 x 14336 31.9 us, 1000 x 4096 x 14336 55.
+// 2048 x 14336 x 4096: 540 cycles a step (512 are the tensor core's), 240 Gop in 84 us in the first milliseconds, 102 once the card's power limit holds the clock at 1.46 GHz; with
+// the quantizer 107 and 127. One CTA with 128 x 256 took 610 cycles a step. 512 x 4096 x 14336, in a graph, quantizer and all, 32 us and (1.73 GHz) 36, 1000 x 4096 x 14336 55 at first.
 #include "lp_mx.cuh"
 #include "lp_mx_mma.cuh"
 #include "lp_tc.cuh"

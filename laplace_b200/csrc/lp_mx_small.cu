@@ -6,8 +6,8 @@
 // core, out of L2 (M x 512 bytes beside 8.7 KB of weights) - and no sum goes through memory: the CTAs of a cluster share out k, and each sends its
 // part of a tile's results straight into the shared memory of the tile's owner, which adds them in the order of k and writes y.
 //
-// One row: 4096 x 1024 3.25 us, 4096 x 4096 5.5, 4096 x 14336 9.8 us (31 MB; a kernel that only copies them from cold memory takes 8), 28672 rows 12.5 us (5 TB/s); eight rows of 4096 x
-// 14336 10.8. With quantizer launch and sums through global memory 8.2, 17.2 and, eight rows, 18.1. Two CTAs an SM, so that the next call's first copies and the
+// One row, in a graph over weights from cold memory: 4096 x 1024 3.4 us, 4096 x 4096 5.3, 4096 x 14336 9.8 us (31 MB, on 112 of 148 SMs; lp_gemv.cu streams 33 MB of Q4_K in
+// 7.7, so it is the ring's bytes in flight that bound it), 28672 rows 12.5 us (5 TB/s); eight rows of 4096 x 14336 10.8. With quantizer launch and sums through global memory 8.2, 17.2 and, eight rows, 18.1. Two CTAs an SM, so that the next call's first copies and the
 // last sums of this one overlap.
 //
 // A cluster of C CTAs takes tiles (128 weight rows x up to 8 tokens) number cluster, cluster + clusters, ...; the i-th of them is owned by CTA i % C.

@@ -291,7 +291,8 @@ def mxfp4_pack(w: torch.Tensor, N: int, K: int, n_experts: int = 1) -> torch.Ten
 
 
 def mxfp4_gemm(x: torch.Tensor, packed: torch.Tensor, M: int, K: int, N: int, y: torch.Tensor | None = None) -> torch.Tensor:
-    """y[m] = W . x[m] with packed MXFP4 weights and x quantized to MXFP8 (laplace_cuda_mxfp4_gemm_dev)."""
+    """y[m] = W . x[m] with packed MXFP4 weights and x quantized to MXFP8 (laplace_cuda_mxfp4_gemm_dev). Up to 8 rows: packed weights that a
+    kernel other than mxfp4_pack's has just written on this stream need a synchronisation before the call (it copies them early)."""
     r = _native and _native.mxfp4_gemm(x, packed, M, K, N, y)
     if r is not None:
         return r
@@ -309,7 +310,8 @@ def mxfp4_gemm(x: torch.Tensor, packed: torch.Tensor, M: int, K: int, N: int, y:
 def mxfp4_moe_grouped(x: torch.Tensor, packed: torch.Tensor, pair_expert: torch.Tensor, pair_row: torch.Tensor | None,
                       n_experts_total: int, K: int, N: int, y: torch.Tensor | None = None) -> torch.Tensor:
     """y[p] = W[pair_expert[p]] . x[pair_row[p]] for (token, expert) pairs in any order, as moe_grouped, with packed MXFP4
-    experts (laplace_cuda_mxfp4_moe_grouped_dev). pair_row None: pair p reads row p. A negative expert leaves its row of y as it was."""
+    experts (laplace_cuda_mxfp4_moe_grouped_dev). pair_row None: pair p reads row p. A negative expert leaves its row of y as it was
+    (without y: undefined)."""
     r = _native and _native.mxfp4_moe_grouped(x, packed, pair_expert, pair_row, n_experts_total, K, N, y)
     if r is not None:
         return r
