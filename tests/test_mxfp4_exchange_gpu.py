@@ -366,3 +366,46 @@ def test_top_4_of_32_experts_of_2880(tokens, gate_up):
     y = device.mxfp4_moe_grouped(_dev(x), device.mxfp4_pack(w, N, K, E), _dev(expert), None if row is None else _dev(row), E, K, N)
     device.sync()
     _close(y, *_experts(x, w, expert, row, E, N, K, np.zeros((4 * tokens, N))), K, f"{tokens} tokens")
+
+
+# ---- a captured call, replayed with other inputs ---------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("P,E,K,N", [(20, 6, 2048, 600), (120, 4, 2048, 1000), (700, 4, 8192, 600), (5000, 40, 256, 300)])
+def test_replayed_with_another_routing(P, E, K, N):
+    """The plan of a call on experts is made on the GPU at every replay: routings from even to all pairs on one expert and to none here, each replay as the call itself."""
+    import torch
+    from laplace_b200 import device
+    rng = np.random.default_rng(1730 + P)
+    packed = device.mxfp4_pack(_weights(1731, E * N, K), N, K, E)
+    x, y = torch.zeros(P, K, device="cuda"), torch.empty(P, N, device="cuda")
+    expert, row = torch.zeros(P, dtype=torch.int32, device="cuda"), torch.zeros(P, dtype=torch.int32, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        device.mxfp4_moe_grouped(x, packed, expert, row, E, K, N, y=y)
+    even = np.arange(P) % E
+    for e in (even, np.full(P, E - 1), np.full(P, -1), np.where(np.arange(P) % 3 == 0, -1, even), rng.choice(E, P, p=rng.dirichlet(np.full(E, 0.3))), np.minimum(even, 1)):
+        x.copy_(_dev(_act(1732 + int(e[0]), P, K)))
+        expert.copy_(_dev(e.astype(np.int32)))
+        row.copy_(_dev(rng.integers(0, P, P).astype(np.int32)))
+        y.fill_(7.0)
+        want = device.mxfp4_moe_grouped(x, packed, expert, row, E, K, N, y=y.clone())
+        g.replay()
+        device.sync()
+        assert torch.equal(y, want) and (y[expert < 0] == 7).all() and not (y[expert >= 0] == 7).all(1).any()
+
+
+@pytest.mark.parametrize("M,K,N", [(3, 4096, 600), (24, 4096, 600), (300, 14336, 2100)])
+def test_replayed_with_other_rows(M, K, N):
+    import torch
+    from laplace_b200 import device
+    packed = device.mxfp4_pack(_weights(1740, N, K), N, K)
+    x, y = torch.zeros(M, K, device="cuda"), torch.empty(M, N, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        device.mxfp4_gemm(x, packed, M, K, N, y=y)
+    for i in range(4):
+        x.copy_(_dev(_act(1741 + i, M, K)))
+        y.fill_(7.0)
+        g.replay()
+        assert torch.equal(y, device.mxfp4_gemm(x, packed, M, K, N))
+    device.sync()
